@@ -8,7 +8,7 @@
  * which wavenet_amd/host/ re-creates on top of this header.
  *
  * Conventions
- *   - every array is fp64; an example is an R x C matrix stored column-major (X(r,c) at
+ *   - every array is fp64 unless its declaration says otherwise; an example is an R x C matrix stored column-major (X(r,c) at
  *     r + c*R, as arma::Mat<double>), examples of a batch are contiguous (X + e*R*C);
  *     R and C are powers of two; a 1D signal of length n is R = n, C = 1
  *     (src/GeneratorBase.cxx:25-31 squeezes {1,n} to {n,1});
@@ -245,6 +245,93 @@ int wn_clear_logs(wn_context* ctx);
  */
 int wn_sparse_cost_grid(wn_context* ctx, const double* X_dev, int B, int R, int C,
                         const double* filters_host, int F, int N, double* S_dev);
+
+/* ---- routed filter bank --------------------------------------------------------------------- */
+/*
+ * Several filters at once, each example under the few it is routed to.  The reference trains one filter at a time and
+ * evaluates a grid of them (Wavenet::costMap, src/Wavenet.cxx:278-324); these entry points have no counterpart there.
+ * A training pass over a batch is
+ *     wn_route               scores of the examples under F filters -> k filters per example and their weights
+ *     wn_forward_routed      Y[e] = sum_j w[e][j] forward(X[e] under filter idx[e][j]), keeping X in 8 bits
+ *     wn_sparse_term_deriv   (or the caller's own cost) -> errors on Y
+ *     wn_backprop_routed     from the 8-bit checkpoint: gradients of the filters, the weights and the input
+ *     wn_route_backward      gradient of the weights -> gradient of the scores
+ * The calls allocate nothing, keep nothing between calls and synchronise nothing: they may be captured into a graph after
+ * one call of the same shape, from any number of contexts at a time.  The device current before a call is current again
+ * after it.  Results are the same bits from run to run.
+ */
+enum { WN_F64 = 0, WN_F32 = 1, WN_F16 = 2, WN_BF16 = 3 };    /* element types */
+enum { WN_SCORE_SOFTMAX = 0, WN_SCORE_SIGMOID = 1 };
+
+#define WN_MAX_EXPERTS 1024 /* filters a router chooses from */
+#define WN_MAX_TOPK 16      /* filters per example */
+#define WN_MAX_GROUPS 64
+
+typedef struct wn_routing {
+    int score;          /* WN_SCORE_SOFTMAX or WN_SCORE_SIGMOID */
+    int k;              /* filters per example, 1 ... min(F, WN_MAX_TOPK) */
+    int groups;         /* equal groups of consecutive filters (1: no groups; at most WN_MAX_GROUPS) */
+    int groups_kept;    /* groups a row chooses from (equal to groups: all) */
+    int renormalise;    /* 1: the weights of a row add up to scale */
+    double scale;       /* of the weights */
+    double score_scale; /* of the scores, not zero; negative where a low score is a good one (sparsity costs) */
+} wn_routing;
+
+/*
+ * scores_dev: T rows of F scores of the given type, score (t, f) at t * row_stride + f * col_stride elements; no two in
+ * one place.  wn_sparse_cost_grid's S_dev (filter by filter) is row_stride 1, col_stride B.
+ *     s = score_scale * score;   p = softmax of the row or sigmoid(s);   c = p + bias[f] (bias_dev may be NULL)
+ *     a group's score is the sum of its two largest c (the largest if there is one); the groups_kept best are kept
+ *     idx[t][0 .. k): the filters of the k largest c left, largest first; equal values in order of the filter
+ *     w[t][j] = scale * p(idx[t][j]), or with renormalise scale * p(idx[t][j]) / sum_j p(idx[t][j])
+ *     counts[f] (counts_dev may be NULL) = number of entries of idx that name f
+ * A filter whose s or c is -inf (or whose bias is NaN) is closed to the row; where fewer than k are open the entries left
+ * over have idx -1 and weight 0.  A row with a NaN or +inf among its s has no answer: idx -1 and weights NaN throughout
+ * (and wn_forward_routed then makes its coefficients NaN).  Computed in 64 bits.
+ */
+int wn_route(wn_context* ctx, const void* scores_dev, int dtype, int T, int F, long long row_stride, long long col_stride,
+             const wn_routing* routing, const double* bias_dev, int* idx_dev, double* w_dev, int* counts_dev);
+/*
+ * dw_dev[T][k]: gradient of the weights -> dscores_dev, the gradient of the scores, in the type and at the strides of the
+ * scores (it may be the same memory).  idx_dev as wn_route left it: the choice itself has no gradient, nor has the bias.
+ * Entries of idx outside 0 ... F - 1 count for nothing; a row without any gets zeros.
+ */
+int wn_route_backward(wn_context* ctx, const void* scores_dev, int dtype, int T, int F, long long row_stride, long long col_stride,
+                      const wn_routing* routing, const int* idx_dev, const double* dw_dev, void* dscores_dev);
+
+/*
+ * 8-bit checkpoints.  A row of n values is cut into blocks of 64 consecutive ones (the last may be shorter);
+ * scale_dev[B][ceil(n / 64)] holds each block's largest magnitude / 127 rounded to float, q_dev[B][n] the whole number
+ * nearest to value / scale (ties to even, within -127 ... 127).  A value reads back as q * scale, at most half a scale
+ * off (more below a scale of 2^-126, where floats are coarser).  A block with a value that is not finite, or too large for
+ * a float scale, reads back as NaN.  dtype and row_stride (elements between rows) describe X_dev.
+ */
+int wn_checkpoint_pack(wn_context* ctx, const void* X_dev, int dtype, int B, int n, long long row_stride, signed char* q_dev,
+                       float* scale_dev);
+int wn_checkpoint_unpack(wn_context* ctx, const signed char* q_dev, const float* scale_dev, int dtype, int B, int n,
+                         long long row_stride, void* X_dev);
+
+/*
+ * wn_forward under routed filters.  filters_dev[F][N]: low-pass taps, on the device (NULL with F = 1 and the context's N:
+ * the context's own filter).  idx_dev[B][k], w_dev[B][k] as wn_route leaves them; idx_dev NULL (k = 1) is filter 0
+ * throughout, w_dev NULL is ones.  An entry outside 0 ... F - 1 names no filter and adds 0 * w.  The same filter may be
+ * named twice.  q_dev and scale_dev (both or neither) receive the checkpoint of X, as wn_checkpoint_pack of B rows of
+ * R * C values.  Examples of up to WN_MAX_FUSED samples.  Y_dev may not overlap the inputs.
+ */
+int wn_forward_routed(wn_context* ctx, const double* X_dev, int B, int R, int C, const double* filters_dev, int F, int N,
+                      const int* idx_dev, const double* w_dev, int k, double* Y_dev, signed char* q_dev, float* scale_dev);
+/*
+ * Its backward pass, at the examples (X_dev) or at the values a checkpoint stands for (q_dev and scale_dev; X_dev NULL):
+ * Delta_dev[B][n] are the errors on Y.
+ *     grad_dev[B][k][N]    w[e][j] * gradient of <Delta, forward(X)> by the taps of filter idx[e][j]
+ *     dfilters_dev[F][N]   sum of the gradients of the entries that name f (may be NULL)
+ *     dw_dev[B][k]         <Delta, forward(X)> under filter idx[e][j] (may be NULL)
+ *     dX_dev[B][n]         errors on the input (may be NULL)
+ * Entries that name no filter have zero grad and dw.
+ */
+int wn_backprop_routed(wn_context* ctx, const double* Delta_dev, const double* X_dev, const signed char* q_dev, const float* scale_dev,
+                       int B, int R, int C, const double* filters_dev, int F, int N, const int* idx_dev, const double* w_dev, int k,
+                       double* grad_dev, double* dfilters_dev, double* dw_dev, double* dX_dev);
 
 /* ---- generators --------------------------------------------------------------------------- */
 /*

@@ -15,9 +15,19 @@ WN_ERR_ARG, WN_ERR_BAD_SHAPE, WN_ERR_BAD_FILTER, WN_ERR_UNSUPPORTED = 1, 2, 3, 4
 WN_ERR_HIP, WN_ERR_COMM, WN_ERR_NONFINITE, WN_ERR_STATE = 5, 6, 7, 8
 WN_MAX_TAPS = 32
 WN_MAX_FUSED = 4096
+WN_F64, WN_F32, WN_F16, WN_BF16 = 0, 1, 2, 3
+WN_SCORE_SOFTMAX, WN_SCORE_SIGMOID = 0, 1
+WN_MAX_EXPERTS, WN_MAX_TOPK, WN_MAX_GROUPS = 1024, 16, 64
 
 _dp = C.POINTER(C.c_double)
 _vp = C.c_void_p
+
+
+class Routing(C.Structure):
+    """wn_routing of include/wavenet_hip.h."""
+    _fields_ = [("score", C.c_int), ("k", C.c_int), ("groups", C.c_int), ("groups_kept", C.c_int), ("renormalise", C.c_int),
+                ("scale", C.c_double), ("score_scale", C.c_double)]
+
 
 # name -> (restype, argtypes); every symbol include/wavenet_hip.h declares
 SIGNATURES = {
@@ -45,6 +55,13 @@ SIGNATURES = {
     "wn_reg_term": (C.c_int, [_dp, C.c_int, C.c_int, _dp]),
     "wn_reg_term_deriv": (C.c_int, [_dp, C.c_int, C.c_int, _dp]),
     "wn_sparse_cost_grid": (C.c_int, [_vp, _vp, C.c_int, C.c_int, C.c_int, _dp, C.c_int, C.c_int, _vp]),
+    "wn_route": (C.c_int, [_vp, _vp, C.c_int, C.c_int, C.c_int, C.c_longlong, C.c_longlong, C.POINTER(Routing), _vp, _vp, _vp, _vp]),
+    "wn_route_backward": (C.c_int, [_vp, _vp, C.c_int, C.c_int, C.c_int, C.c_longlong, C.c_longlong, C.POINTER(Routing), _vp, _vp, _vp]),
+    "wn_checkpoint_pack": (C.c_int, [_vp, _vp, C.c_int, C.c_int, C.c_int, C.c_longlong, _vp, _vp]),
+    "wn_checkpoint_unpack": (C.c_int, [_vp, _vp, _vp, C.c_int, C.c_int, C.c_int, C.c_longlong, _vp]),
+    "wn_forward_routed": (C.c_int, [_vp, _vp, C.c_int, C.c_int, C.c_int, _vp, C.c_int, C.c_int, _vp, _vp, C.c_int, _vp, _vp, _vp]),
+    "wn_backprop_routed": (C.c_int, [_vp, _vp, _vp, _vp, _vp, C.c_int, C.c_int, C.c_int, _vp, C.c_int, C.c_int, _vp, _vp, C.c_int,
+                                     _vp, _vp, _vp, _vp]),
     "wn_generate_uniform": (C.c_int, [_vp, C.c_ulonglong, C.c_longlong, C.c_int, C.c_int, C.c_int, _vp]),
     "wn_generate_needle": (C.c_int, [_vp, C.c_ulonglong, C.c_longlong, C.c_int, C.c_int, C.c_int, C.c_double, _vp]),
     "wn_generate_calorimeter": (C.c_int, [_vp, C.c_ulonglong, C.c_longlong, C.c_int, C.c_int, C.c_int,
@@ -125,6 +142,27 @@ def _addr(x):
 def _hd(a):
     a = np.ascontiguousarray(a, dtype=np.float64)
     return a, a.ctypes.data_as(_dp)
+
+
+_TYPE_CODES = {"float64": WN_F64, "float32": WN_F32, "float16": WN_F16, "bfloat16": WN_BF16}
+
+
+def _type_name(x):
+    return str(x.dtype).rsplit(".", 1)[-1]
+
+
+def _dtype_code(x, dtype):
+    """Element type code: of a tensor, or of an address by the code or name given with it (default float64)."""
+    if x is not None and not isinstance(x, int):
+        name = _type_name(x)
+        if name not in _TYPE_CODES:
+            raise ValueError(f"element type {name} is not one of {sorted(_TYPE_CODES)}")
+        if dtype is not None and _TYPE_CODES[name] != _TYPE_CODES.get(dtype, dtype):
+            raise ValueError(f"element type is {name}, not {dtype}")
+        return _TYPE_CODES[name]
+    if dtype is None:
+        return WN_F64
+    return _TYPE_CODES.get(dtype, dtype)
 
 
 # --- host-only entry points ----------------------------------------------------------------------
@@ -244,6 +282,123 @@ class Context:
         assert f.ndim == 2
         self._check(self.lib.wn_sparse_cost_grid(self._h, _addr(X), B, R, Cc, f.ctypes.data_as(_dp), f.shape[0],
                                                  f.shape[1], _addr(S)))
+
+    # routed filter bank ---------------------------------------------------------------------------
+    def _buffer(self, name, x, count, *types, span=None):
+        """Address of an argument.  A tensor has to lie on the context's GPU, hold `count` elements (or with `span` reach
+        that far from its first) of one of the types, densely; an address is taken as it is."""
+        if x is None or isinstance(x, int):
+            return x
+        if not x.is_cuda or x.device.index != self.device:
+            raise ValueError(f"{name} is on {x.device}, the context on GPU {self.device}")
+        if types and _type_name(x) not in types:
+            raise ValueError(f"{name} holds {_type_name(x)}, not {' or '.join(types)}")
+        if span is None:
+            if not x.is_contiguous():
+                raise ValueError(f"{name} is not contiguous")
+            if x.numel() < count:
+                raise ValueError(f"{name} holds {x.numel()} elements, {count} are needed")
+        else:
+            held = x.untyped_storage().nbytes() // x.element_size() - x.storage_offset()
+            if held < span:
+                raise ValueError(f"{name} ends {held} elements after its start, {span} are needed")
+        return x.data_ptr()
+
+    @staticmethod
+    def _routing(k, score, groups, groups_kept, renormalise, scale, score_scale):
+        code = {"softmax": WN_SCORE_SOFTMAX, "sigmoid": WN_SCORE_SIGMOID}.get(score, score)
+        if not isinstance(code, int):
+            raise ValueError(f"score is {score!r}, not 'softmax' or 'sigmoid'")
+        return Routing(code, int(k), int(groups), int(groups if groups_kept is None else groups_kept), int(bool(renormalise)),
+                       float(scale), float(score_scale))
+
+    def route(self, scores, T, F, idx, w, k=1, score="softmax", bias=None, groups=1, groups_kept=None, renormalise=True,
+              scale=1.0, score_scale=1.0, counts=None, row_stride=None, col_stride=1, dtype=None):
+        """wn_route: the k filters of each of T rows of F scores, and their weights.
+
+        scores: tensor (its element type is used) or address (dtype: "float64", "float32", "float16" or "bfloat16");
+        score (t, f) lies t * row_stride + f * col_stride elements from the start (default: dense rows).
+        idx: int32 [T][k], w: float64 [T][k], bias: float64 [F], counts: int32 [F]."""
+        rs = F * col_stride if row_stride is None else row_stride
+        span = (T - 1) * rs + (F - 1) * col_stride + 1 if T > 0 else 0
+        r = self._routing(k, score, groups, groups_kept, renormalise, scale, score_scale)
+        self._check(self.lib.wn_route(
+            self._h, self._buffer("scores", scores, 0, span=span), _dtype_code(scores, dtype), T, F, rs, col_stride, C.byref(r),
+            self._buffer("bias", bias, F, "float64"), self._buffer("idx", idx, T * k, "int32"),
+            self._buffer("w", w, T * k, "float64"), self._buffer("counts", counts, F, "int32")))
+
+    def route_backward(self, scores, T, F, idx, dw, dscores, k=1, score="softmax", groups=1, groups_kept=None, renormalise=True,
+                       scale=1.0, score_scale=1.0, row_stride=None, col_stride=1, dtype=None):
+        """wn_route_backward: gradient dw of the weights -> gradient of the scores, laid out as the scores."""
+        rs = F * col_stride if row_stride is None else row_stride
+        span = (T - 1) * rs + (F - 1) * col_stride + 1 if T > 0 else 0
+        r = self._routing(k, score, groups, groups_kept, renormalise, scale, score_scale)
+        code = _dtype_code(scores, dtype)
+        if _dtype_code(dscores, dtype if isinstance(dscores, int) else None) != code and dscores is not None and not isinstance(dscores, int):
+            raise ValueError("dscores and scores differ in type")
+        self._check(self.lib.wn_route_backward(
+            self._h, self._buffer("scores", scores, 0, span=span), code, T, F, rs, col_stride, C.byref(r),
+            self._buffer("idx", idx, T * k, "int32"), self._buffer("dw", dw, T * k, "float64"),
+            self._buffer("dscores", dscores, 0, span=span)))
+
+    def checkpoint_pack(self, X, B, n, q, scales, row_stride=None, dtype=None):
+        """wn_checkpoint_pack: B rows of n values as int8 q[B][n] and float32 scales[B][ceil(n / 64)]."""
+        rs = n if row_stride is None else row_stride
+        self._check(self.lib.wn_checkpoint_pack(
+            self._h, self._buffer("X", X, 0, span=(B - 1) * rs + n if B > 0 else 0), _dtype_code(X, dtype), B, n, rs,
+            self._buffer("q", q, B * n, "int8"), self._buffer("scales", scales, B * -(-n // 64), "float32")))
+
+    def checkpoint_unpack(self, q, scales, B, n, X, row_stride=None, dtype=None):
+        """wn_checkpoint_unpack: the values a checkpoint stands for, in the type of X."""
+        rs = n if row_stride is None else row_stride
+        self._check(self.lib.wn_checkpoint_unpack(
+            self._h, self._buffer("q", q, B * n, "int8"), self._buffer("scales", scales, B * -(-n // 64), "float32"),
+            _dtype_code(X, dtype), B, n, rs, self._buffer("X", X, 0, span=(B - 1) * rs + n if B > 0 else 0)))
+
+    def _bank(self, filters, F, N):
+        """(filters, F, N): a tensor [F][N] says both numbers; None is the context's own filter."""
+        if filters is None and N is None:
+            n = C.c_int(0)
+            self._check(self.lib.wn_get_filter(self._h, None, C.byref(n)))
+            return None, 1 if F is None else F, n.value
+        if filters is not None and not isinstance(filters, int) and filters.dim() == 2:
+            F = filters.shape[0] if F is None else F
+            N = filters.shape[1] if N is None else N
+        if F is None or N is None:
+            raise ValueError("the number of filters and of taps is not known: pass a tensor [F][N], or F and N")
+        return self._buffer("filters", filters, F * N, "float64"), F, N
+
+    @staticmethod
+    def _entries(idx, w, k):
+        for x in (idx, w):
+            if k is None and x is not None and not isinstance(x, int) and x.dim() == 2:
+                k = x.shape[1]
+        return 1 if k is None else k
+
+    def forward_routed(self, X, B, R, Cc, filters, idx, w, Y, k=None, q=None, scales=None, F=None, N=None):
+        """wn_forward_routed: Y[e] = sum_j w[e][j] forward(X[e] under filters[idx[e][j]]).
+
+        filters: float64 [F][N] (None: the context's filter); idx: int32 [B][k] (None: filter 0); w: float64 [B][k]
+        (None: ones); q, scales: where to keep the checkpoint of X, if wanted."""
+        filters, F, N = self._bank(filters, F, N)
+        k, n = self._entries(idx, w, k), R * Cc
+        self._check(self.lib.wn_forward_routed(
+            self._h, self._buffer("X", X, B * n, "float64"), B, R, Cc, filters, F, N, self._buffer("idx", idx, B * k, "int32"),
+            self._buffer("w", w, B * k, "float64"), k, self._buffer("Y", Y, B * n, "float64"), self._buffer("q", q, B * n, "int8"),
+            self._buffer("scales", scales, B * -(-n // 64), "float32")))
+
+    def backprop_routed(self, Delta, B, R, Cc, filters, idx, w, grad, X=None, q=None, scales=None, dfilters=None, dw=None, dX=None,
+                        k=None, F=None, N=None):
+        """wn_backprop_routed: errors Delta on Y -> grad[B][k][N], dfilters[F][N], dw[B][k], dX[B][n], at the examples X or at
+        the checkpoint (q, scales) that forward_routed or checkpoint_pack kept."""
+        filters, F, N = self._bank(filters, F, N)
+        k, n = self._entries(idx, w, k), R * Cc
+        self._check(self.lib.wn_backprop_routed(
+            self._h, self._buffer("Delta", Delta, B * n, "float64"), self._buffer("X", X, B * n, "float64"),
+            self._buffer("q", q, B * n, "int8"), self._buffer("scales", scales, B * -(-n // 64), "float32"), B, R, Cc, filters, F, N,
+            self._buffer("idx", idx, B * k, "int32"), self._buffer("w", w, B * k, "float64"), k,
+            self._buffer("grad", grad, B * k * N, "float64"), self._buffer("dfilters", dfilters, F * N, "float64"),
+            self._buffer("dw", dw, B * k, "float64"), self._buffer("dX", dX, B * n, "float64")))
 
     # generators ---------------------------------------------------------------------------------
     def generate_uniform(self, X, B, R, Cc, seed=1, first=0):

@@ -1,0 +1,148 @@
+// Shared by the routed filter bank (wn_route.hip, wn_checkpoint.hip, wn_bank.hip, wn_bank_np.hip): argument blocks,
+// element types, the 8-bit checkpoint format, and the host-side frame of an entry point.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <exception>
+#include <string>
+
+#include "wavenet_hip.h"
+#include "wn_device.h"
+#include "wn_internal.h"
+
+namespace wn {
+
+// ---- entry points -------------------------------------------------------------------------------------
+
+// The context's device for the length of a call; the caller's device is current again afterwards.
+struct DeviceScope {
+    int before = -1;
+    bool moved = false;
+    hipError_t status;
+    explicit DeviceScope(int device) {
+        status = hipGetDevice(&before);
+        if (status == hipSuccess && before != device) {
+            status = hipSetDevice(device);
+            moved = status == hipSuccess;
+        }
+    }
+    ~DeviceScope() {
+        if (moved) (void)hipSetDevice(before);
+    }
+};
+
+// Runs the body of an entry point: null context, device, and no exception past the C boundary.
+template <class Body>
+int entry(wn_context* ctx, Body body) noexcept {
+    if (!ctx) return WN_ERR_ARG;
+    try {
+        DeviceScope scope(ctx->device);
+        WN_HIP(ctx, scope.status);
+        return body();
+    } catch (const std::exception& e) {
+        try {
+            return fail(ctx, WN_ERR_HIP, e.what());
+        } catch (...) {
+        }
+    } catch (...) {
+    }
+    return WN_ERR_HIP;
+}
+
+template <class Args>
+int launch_kernel(wn_context* ctx, const void* func, unsigned grid, unsigned threads, size_t shmem, Args& args) {
+    if (!func) return fail(ctx, WN_ERR_UNSUPPORTED, "no kernel compiled for this configuration");
+    if (shmem > 64 * 1024) {
+        size_t& have = ctx->lds_configured[func];
+        if (have < shmem) {
+            WN_HIP(ctx, hipFuncSetAttribute(func, hipFuncAttributeMaxDynamicSharedMemorySize, (int)shmem));
+            have = shmem;
+        }
+    }
+    void* p[] = {&args};
+    WN_HIP(ctx, hipLaunchKernel(func, dim3(grid), dim3(threads), p, shmem, ctx->stream));
+    return WN_OK;
+}
+
+inline bool aligned_to(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
+inline size_t element_bytes(int dtype) {
+    switch (dtype) {
+        case WN_F64: return 8;
+        case WN_F32: return 4;
+        case WN_F16: case WN_BF16: return 2;
+    }
+    return 0;
+}
+
+// ---- element types: everything is computed in 64 bits, so that reading is exact and writing rounds once ----------
+
+struct f16_bits { unsigned short v; };
+struct bf16_bits { unsigned short v; };
+
+__device__ __forceinline__ double widen(double v) { return v; }
+__device__ __forceinline__ double widen(float v) { return v; }
+__device__ __forceinline__ double widen(f16_bits v) { return (double)(float)__builtin_bit_cast(_Float16, v.v); }
+__device__ __forceinline__ double widen(bf16_bits v) { return (double)__builtin_bit_cast(float, (unsigned)v.v << 16); }
+
+// d in 24 bits, rounded to odd: truncated, with the last bit set if anything was cut off.  Rounding that to 13 bits or
+// fewer gives what rounding d itself gives, which rounding to the nearest float first does not.
+__device__ __forceinline__ float round_to_odd(double d) {
+    const float f = (float)d;
+    if ((double)f == d || d != d) return f;
+    unsigned u = __builtin_bit_cast(unsigned, f);
+    if (__builtin_fabs((double)f) > __builtin_fabs(d)) u -= 1;
+    return __builtin_bit_cast(float, u | 1u);
+}
+template <class S> __device__ __forceinline__ S narrow(double d);
+template <> __device__ __forceinline__ double narrow<double>(double d) { return d; }
+template <> __device__ __forceinline__ float narrow<float>(double d) { return (float)d; }
+template <> __device__ __forceinline__ f16_bits narrow<f16_bits>(double d) {
+    return {__builtin_bit_cast(unsigned short, (_Float16)round_to_odd(d))};
+}
+template <> __device__ __forceinline__ bf16_bits narrow<bf16_bits>(double d) {
+    const unsigned u = __builtin_bit_cast(unsigned, round_to_odd(d));
+    if (d != d) return {(unsigned short)((u >> 16) | 0x40u)};
+    return {(unsigned short)((u + 0x7FFFu + ((u >> 16) & 1u)) >> 16)};
+}
+
+// ---- 8-bit checkpoints ------------------------------------------------------------------------------------
+// Blocks of CKPT_BLOCK consecutive values share a float scale = largest magnitude / 127; a value is kept as the whole
+// number q nearest to value / scale and read back as q * scale (7 bits times 24 bits: exact in a double).
+
+constexpr int CKPT_BLOCK = 64;
+
+// amax: the block's largest magnitude, any value not finite already replaced by a NaN
+__device__ __forceinline__ float ckpt_scale(double amax) { return (float)(amax / 127.0); }
+__device__ __forceinline__ int ckpt_quantise(double x, float scale) {
+    if (!(scale > 0.0f && scale <= 3.402823466e38f)) return 0;   // nothing there, or a block that reads back as NaN
+    const double r = __builtin_rint(x / (double)scale);
+    return (int)__builtin_fmin(127.0, __builtin_fmax(-127.0, r));
+}
+// |x|, or a NaN for what no scale can hold; the larger of two such magnitudes, NaN winning
+__device__ __forceinline__ double ckpt_magnitude(double x) { return __builtin_fabs(x) <= 1.7976931348623157e308 ? __builtin_fabs(x) : __builtin_nan(""); }
+__device__ __forceinline__ double ckpt_max(double a, double b) { return (a > b || a != a) ? a : b; }
+
+// ---- routed transforms --------------------------------------------------------------------------------------
+
+constexpr int BANK_MAX_TOPK = WN_MAX_TOPK;
+
+struct BankArgs {
+    int B, lgR, lgC, k, F, N;
+    const double* filters;   // [F][N] taps
+    const int* idx;          // [B][k], null: every entry names filter 0
+    const double* w;         // [B][k], null: ones
+    const double* X;         // [B][n] examples (forward; backward unless a checkpoint is given)
+    const signed char* q;    // backward: checkpoint of X, [B][n] whole numbers and one scale per block
+    const float* qs;
+    signed char* q_out;      // forward: checkpoint to write, optional
+    float* qs_out;
+    double* Y;               // forward: [B][n]
+    const double* D;         // backward: errors on the coefficients
+    double* dX;              // [B][n], optional
+    double* dw;              // [B][k], optional
+    double* grad;            // [B][k][N]
+};
+
+}  // namespace wn

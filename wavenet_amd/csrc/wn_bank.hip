@@ -1,0 +1,161 @@
+// Routed filter bank: wn_forward_routed, wn_backprop_routed.
+#include <algorithm>
+
+#include "wn_bank.h"
+
+extern "C" const void* wn_kernel_bank_np2(int kind, int sc);
+extern "C" const void* wn_kernel_bank_np4(int kind, int sc);
+extern "C" const void* wn_kernel_bank_np8(int kind, int sc);
+extern "C" const void* wn_kernel_bank_np16(int kind, int sc);
+extern "C" const void* wn_kernel_bank_np32(int kind, int sc);
+
+namespace wn {
+
+struct BankReduceArgs {
+    const int* idx;
+    const double* grad;
+    double* out;
+    long long entries;
+    int N;
+};
+
+// dfilters[f] = sum of the gradients of the entries that name f.  A workgroup per filter; thread t adds entries t,
+// t + 256, ... in order, then the threads are added in a fixed tree: the same bits from run to run.
+template <int NP>
+__global__ __launch_bounds__(256) void k_bank_reduce(BankReduceArgs A) {
+    __shared__ double red[4 * NP];
+    const int f = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+    double s[NP];
+#pragma unroll
+    for (int t = 0; t < NP; t++) s[t] = 0;
+    for (long long i = tid; i < A.entries; i += 256) {
+        if ((A.idx ? A.idx[i] : 0) == f) {
+            const double* g = A.grad + i * A.N;
+#pragma unroll
+            for (int t = 0; t < NP; t++) s[t] += t < A.N ? g[t] : 0.0;
+        }
+    }
+    const double mine = wave_scatter_sums<NP>(s, lane);
+    if (lane < NP) red[(tid >> 6) * NP + lane] = mine;
+    __syncthreads();
+    if (tid < A.N) A.out[(size_t)f * A.N + tid] = red[tid] + red[NP + tid] + red[2 * NP + tid] + red[3 * NP + tid];
+}
+
+}  // namespace wn
+
+namespace {
+
+using wn::fail;
+
+struct SizeClass { int T, Q; };
+const SizeClass kSizeClasses[5] = {{64, 1}, {64, 3}, {64, 4}, {256, 3}, {512, 3}};
+
+int size_class(long long n) { return n <= 128 ? 0 : n <= 512 ? 1 : n <= 1024 ? 2 : n <= 2048 ? 3 : n <= 4096 ? 4 : -1; }
+
+int ilog2_exact(int v) { return (v < 1 || (v & (v - 1))) ? -1 : __builtin_ctz((unsigned)v); }
+
+const void* kernel_for(int NP, int kind, int sc) {
+    switch (NP) {
+        case 2: return wn_kernel_bank_np2(kind, sc);
+        case 4: return wn_kernel_bank_np4(kind, sc);
+        case 8: return wn_kernel_bank_np8(kind, sc);
+        case 16: return wn_kernel_bank_np16(kind, sc);
+        case 32: return wn_kernel_bank_np32(kind, sc);
+    }
+    return nullptr;
+}
+const void* reduce_for(int NP) {
+    switch (NP) {
+        case 2: return (const void*)&wn::k_bank_reduce<2>;
+        case 4: return (const void*)&wn::k_bank_reduce<4>;
+        case 8: return (const void*)&wn::k_bank_reduce<8>;
+        case 16: return (const void*)&wn::k_bank_reduce<16>;
+    }
+    return (const void*)&wn::k_bank_reduce<32>;
+}
+
+// What both directions check: shape, bank, routing.  Fills A and the compiled tap count.
+int check_bank(wn_context* ctx, int B, int R, int C, const double* filters, int F, int N, const int* idx, const double* w, int k,
+               wn::BankArgs& A, int& NP, int& sc) {
+    if (B < 0) return fail(ctx, WN_ERR_ARG, "negative batch size");
+    A.lgR = ilog2_exact(R);
+    A.lgC = ilog2_exact(C);
+    if (A.lgR < 0 || A.lgC < 0)
+        return fail(ctx, WN_ERR_BAD_SHAPE, "shape {" + std::to_string(R) + ", " + std::to_string(C) + "} is not radix 2");
+    if (filters) {
+        if (F < 1) return fail(ctx, WN_ERR_ARG, "no filters");
+        if (N <= 0) return fail(ctx, WN_ERR_BAD_FILTER, "Input filter is empty.");
+        if (N % 2) return fail(ctx, WN_ERR_BAD_FILTER, "Input filter length is not a multiple of 2.");
+        A.filters = filters;
+    } else {
+        if (!ctx->has_filter) return fail(ctx, WN_ERR_STATE, "no filter set");
+        if (F != 1 || N != ctx->N) return fail(ctx, WN_ERR_ARG, "the context holds one filter of " + std::to_string(ctx->N) + " taps");
+        A.filters = ctx->dfilt->a_true;
+    }
+    if (N > WN_MAX_TAPS) return fail(ctx, WN_ERR_UNSUPPORTED, "filter length " + std::to_string(N) + " exceeds " + std::to_string(WN_MAX_TAPS));
+    NP = 2;
+    while (NP < N) NP *= 2;
+    if (k < 1 || k > WN_MAX_TOPK) return fail(ctx, WN_ERR_ARG, "k is " + std::to_string(k) + ", not 1 ... " + std::to_string(WN_MAX_TOPK));
+    if (!idx && k != 1 && B > 0) return fail(ctx, WN_ERR_ARG, "without indices every example has one filter, k is " + std::to_string(k));
+    const long long n = 1LL << (A.lgR + A.lgC);
+    sc = size_class(n);
+    if (sc < 0)
+        return fail(ctx, WN_ERR_UNSUPPORTED, "routed transforms: examples of " + std::to_string(n) + " samples exceed the " + std::to_string(WN_MAX_FUSED));
+    if (!wn::aligned_to(filters, 8) || !wn::aligned_to(idx, 4) || !wn::aligned_to(w, 8)) return fail(ctx, WN_ERR_ARG, "misaligned pointer");
+    A.B = B; A.k = k; A.F = F; A.N = N; A.idx = idx; A.w = w;
+    return WN_OK;
+}
+
+unsigned grid_for(wn_context* ctx, int B) { return (unsigned)std::min<long long>(B, (long long)ctx->numCU * 32); }
+
+}  // namespace
+
+extern "C" {
+
+int wn_forward_routed(wn_context* ctx, const double* X_dev, int B, int R, int C, const double* filters_dev, int F, int N,
+                      const int* idx_dev, const double* w_dev, int k, double* Y_dev, signed char* q_dev, float* scale_dev) {
+    return wn::entry(ctx, [&]() -> int {
+        wn::BankArgs A = {};
+        int NP, sc;
+        int rc = check_bank(ctx, B, R, C, filters_dev, F, N, idx_dev, w_dev, k, A, NP, sc);
+        if (rc || B == 0) return rc;
+        if (!X_dev || !Y_dev) return fail(ctx, WN_ERR_ARG, "null pointer");
+        if (!q_dev != !scale_dev) return fail(ctx, WN_ERR_ARG, "a checkpoint is values and scales");
+        if (!wn::aligned_to(X_dev, 8) || !wn::aligned_to(Y_dev, 8) || !wn::aligned_to(scale_dev, 4)) return fail(ctx, WN_ERR_ARG, "misaligned pointer");
+        A.X = X_dev; A.Y = Y_dev; A.q_out = q_dev; A.qs_out = scale_dev;
+        const size_t n = (size_t)1 << (A.lgR + A.lgC);
+        const size_t shmem = (A.lgC > 0 ? 4 : 3) * n * sizeof(double);
+        return wn::launch_kernel(ctx, kernel_for(NP, 0, sc), grid_for(ctx, B), kSizeClasses[sc].T, shmem, A);
+    });
+}
+
+int wn_backprop_routed(wn_context* ctx, const double* Delta_dev, const double* X_dev, const signed char* q_dev, const float* scale_dev,
+                       int B, int R, int C, const double* filters_dev, int F, int N, const int* idx_dev, const double* w_dev, int k,
+                       double* grad_dev, double* dfilters_dev, double* dw_dev, double* dX_dev) {
+    return wn::entry(ctx, [&]() -> int {
+        wn::BankArgs A = {};
+        int NP, sc;
+        int rc = check_bank(ctx, B, R, C, filters_dev, F, N, idx_dev, w_dev, k, A, NP, sc);
+        if (rc) return rc;
+        if (B > 0) {
+            if (!Delta_dev || !grad_dev) return fail(ctx, WN_ERR_ARG, "null pointer");
+            if (!q_dev != !scale_dev) return fail(ctx, WN_ERR_ARG, "a checkpoint is values and scales");
+            if (!X_dev == !q_dev) return fail(ctx, WN_ERR_ARG, "either the examples or their checkpoint");
+            if (!wn::aligned_to(Delta_dev, 8) || !wn::aligned_to(X_dev, 8) || !wn::aligned_to(scale_dev, 4) || !wn::aligned_to(grad_dev, 8) ||
+                !wn::aligned_to(dw_dev, 8) || !wn::aligned_to(dX_dev, 8))
+                return fail(ctx, WN_ERR_ARG, "misaligned pointer");
+            A.D = Delta_dev; A.X = X_dev; A.q = q_dev; A.qs = scale_dev; A.grad = grad_dev; A.dw = dw_dev; A.dX = dX_dev;
+            const SizeClass& S = kSizeClasses[sc];
+            const size_t n = (size_t)1 << (A.lgR + A.lgC);
+            const size_t shmem = ((A.lgC > 0 ? 4 : 3) * n + (size_t)(S.T / 64) * NP + 2) * sizeof(double);
+            rc = wn::launch_kernel(ctx, kernel_for(NP, 1, sc), grid_for(ctx, B), S.T, shmem, A);
+            if (rc) return rc;
+        }
+        if (!dfilters_dev) return WN_OK;
+        if (!wn::aligned_to(dfilters_dev, 8)) return fail(ctx, WN_ERR_ARG, "misaligned pointer");
+        wn::BankReduceArgs S = {idx_dev, grad_dev, dfilters_dev, (long long)B * k, N};
+        return wn::launch_kernel(ctx, reduce_for(NP), (unsigned)F, 256, 0, S);
+    });
+}
+
+}  // extern "C"

@@ -1,0 +1,22 @@
+// Instantiates the routed transforms for one compiled tap count (-DWN_NP=2|4|8|16|32) and exports their addresses:
+// kind 0 forward, 1 backward; size class as in wn_fused_np.hip.
+#include "wn_bank_kernels.h"
+
+#ifndef WN_NP
+#error "compile with -DWN_NP=<taps>"
+#endif
+
+#define WN_CAT2(a, b) a##b
+#define WN_CAT(a, b) WN_CAT2(a, b)
+#define WN_KERNELS(T, Q) return kind ? (const void*)&wn::k_bank_backward<WN_NP, T, Q> : (const void*)&wn::k_bank_forward<WN_NP, T, Q>
+
+extern "C" const void* WN_CAT(wn_kernel_bank_np, WN_NP)(int kind, int sc) {
+    switch (sc) {
+        case 0: WN_KERNELS(64, 1);
+        case 1: WN_KERNELS(64, 3);
+        case 2: WN_KERNELS(64, 4);
+        case 3: WN_KERNELS(256, 3);
+        case 4: WN_KERNELS(512, 3);
+    }
+    return nullptr;
+}
