@@ -120,6 +120,13 @@ __device__ __forceinline__ int ckpt_quantise(double x, float scale) {
     const double r = __builtin_rint(x / (double)scale);
     return (int)__builtin_fmin(127.0, __builtin_fmax(-127.0, r));
 }
+// The same from inv = 1 / scale: x * inv is within 2^-45 of x / scale, so that it rounds alike unless it lies next to the
+// middle between two whole numbers, and only then is the division made.
+__device__ __forceinline__ int ckpt_quantise_fast(double x, float scale, double inv) {
+    const double t = x * inv, r = __builtin_rint(t);
+    if (__builtin_fabs(t - r) <= 0.499999 && __builtin_fabs(r) <= 127.0) return (int)r;
+    return ckpt_quantise(x, scale);                        // NaN and what does not fit come here too
+}
 // |x|, or a NaN for what no scale can hold; the larger of two such magnitudes, NaN winning
 __device__ __forceinline__ double ckpt_magnitude(double x) { return __builtin_fabs(x) <= 1.7976931348623157e308 ? __builtin_fabs(x) : __builtin_nan(""); }
 __device__ __forceinline__ double ckpt_max(double a, double b) { return (a > b || a != a) ? a : b; }

@@ -8,8 +8,15 @@ extern "C" const void* wn_kernel_bank_np4(int kind, int sc);
 extern "C" const void* wn_kernel_bank_np8(int kind, int sc);
 extern "C" const void* wn_kernel_bank_np16(int kind, int sc);
 extern "C" const void* wn_kernel_bank_np32(int kind, int sc);
+extern "C" const void* wn_kernel_bank64_np2(int kind);
+extern "C" const void* wn_kernel_bank64_np4(int kind);
+extern "C" const void* wn_kernel_bank64_np8(int kind);
+extern "C" const void* wn_kernel_bank64_np16(int kind);
+extern "C" const void* wn_kernel_bank64_np32(int kind);
 
 namespace wn {
+
+constexpr size_t BANK_TILE = (64 * 65 + 1) * sizeof(double);   // LDS per wave of the 64x64 kernels: a tile and a weight
 
 struct BankReduceArgs {
     const int* idx;
@@ -64,6 +71,16 @@ const void* kernel_for(int NP, int kind, int sc) {
     }
     return nullptr;
 }
+const void* kernel64_for(int NP, int kind) {
+    switch (NP) {
+        case 2: return wn_kernel_bank64_np2(kind);
+        case 4: return wn_kernel_bank64_np4(kind);
+        case 8: return wn_kernel_bank64_np8(kind);
+        case 16: return wn_kernel_bank64_np16(kind);
+        case 32: return wn_kernel_bank64_np32(kind);
+    }
+    return nullptr;
+}
 const void* reduce_for(int NP) {
     switch (NP) {
         case 2: return (const void*)&wn::k_bank_reduce<2>;
@@ -108,6 +125,12 @@ int check_bank(wn_context* ctx, int B, int R, int C, const double* filters, int 
 
 unsigned grid_for(wn_context* ctx, int B) { return (unsigned)std::min<long long>(B, (long long)ctx->numCU * 32); }
 
+// 64x64 examples: a workgroup per example, a wave per filter, up to the four waves whose tiles fit a CU.
+int launch64(wn_context* ctx, int NP, int kind, wn::BankArgs& A) {
+    const int waves = std::min(A.k, 4);
+    return wn::launch_kernel(ctx, kernel64_for(NP, kind), grid_for(ctx, A.B), 64 * waves, waves * wn::BANK_TILE, A);
+}
+
 }  // namespace
 
 extern "C" {
@@ -123,6 +146,7 @@ int wn_forward_routed(wn_context* ctx, const double* X_dev, int B, int R, int C,
         if (!q_dev != !scale_dev) return fail(ctx, WN_ERR_ARG, "a checkpoint is values and scales");
         if (!wn::aligned_to(X_dev, 8) || !wn::aligned_to(Y_dev, 8) || !wn::aligned_to(scale_dev, 4)) return fail(ctx, WN_ERR_ARG, "misaligned pointer");
         A.X = X_dev; A.Y = Y_dev; A.q_out = q_dev; A.qs_out = scale_dev;
+        if (A.lgR == 6 && A.lgC == 6 && ctx->wave64) return launch64(ctx, NP, 0, A);
         const size_t n = (size_t)1 << (A.lgR + A.lgC);
         const size_t shmem = (A.lgC > 0 ? 4 : 3) * n * sizeof(double);
         return wn::launch_kernel(ctx, kernel_for(NP, 0, sc), grid_for(ctx, B), kSizeClasses[sc].T, shmem, A);
@@ -148,7 +172,8 @@ int wn_backprop_routed(wn_context* ctx, const double* Delta_dev, const double* X
             const SizeClass& S = kSizeClasses[sc];
             const size_t n = (size_t)1 << (A.lgR + A.lgC);
             const size_t shmem = ((A.lgC > 0 ? 4 : 3) * n + (size_t)(S.T / 64) * NP + 2) * sizeof(double);
-            rc = wn::launch_kernel(ctx, kernel_for(NP, 1, sc), grid_for(ctx, B), S.T, shmem, A);
+            rc = (A.lgR == 6 && A.lgC == 6 && ctx->wave64) ? launch64(ctx, NP, q_dev ? 2 : 1, A)
+                                                           : wn::launch_kernel(ctx, kernel_for(NP, 1, sc), grid_for(ctx, B), S.T, shmem, A);
             if (rc) return rc;
         }
         if (!dfilters_dev) return WN_OK;

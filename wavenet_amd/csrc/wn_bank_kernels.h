@@ -30,11 +30,11 @@ __device__ __forceinline__ bool bank_entry(const BankArgs& A, int e, int j, int&
 }
 
 // Tap k' = k + d of the gradient from the window sums (reduce_gradient, wn_kernels.h, without a FilterDev): thread k'
-// returns the sum over the workgroup, the threads beyond NP return 0.
+// returns the sum over the workgroup, the threads beyond NP return 0.  sign: that of the high-pass window sums.
 template <int NP, int T>
-__device__ __forceinline__ double bank_gradient(const double (&gL)[NP], const double (&gH)[NP], int N, double* red, int tid) {
+__device__ __forceinline__ double bank_gradient(const double (&gL)[NP], const double (&gH)[NP], int N, double* red, int tid, double sign = 1.0) {
     const int d = (NP - N) / 2;
-    const double sg = ((N - 1 + d) & 1) ? -1.0 : 1.0;      // (-1)^(N-1-k), k = k' - d
+    const double sg = ((N - 1 + d) & 1) ? -sign : sign;      // (-1)^(N-1-k), k = k' - d
     double cp[NP];
 #pragma unroll
     for (int kp = 0; kp < NP; kp++) cp[kp] = gL[kp] + ((kp & 1) ? -sg : sg) * gH[NP - 1 - kp];

@@ -1,6 +1,7 @@
 // Instantiates the routed transforms for one compiled tap count (-DWN_NP=2|4|8|16|32) and exports their addresses:
-// kind 0 forward, 1 backward; size class as in wn_fused_np.hip.
-#include "wn_bank_kernels.h"
+// kind 0 forward, 1 backward; size class as in wn_fused_np.hip.  wn_kernel_bank64_np<taps>: the kernels of 64x64 examples, kind
+// 0 forward, 1 backward from the examples, 2 backward from a checkpoint.
+#include "wn_bank64.h"
 
 #ifndef WN_NP
 #error "compile with -DWN_NP=<taps>"
@@ -17,6 +18,15 @@ extern "C" const void* WN_CAT(wn_kernel_bank_np, WN_NP)(int kind, int sc) {
         case 2: WN_KERNELS(64, 4);
         case 3: WN_KERNELS(256, 3);
         case 4: WN_KERNELS(512, 3);
+    }
+    return nullptr;
+}
+
+extern "C" const void* WN_CAT(wn_kernel_bank64_np, WN_NP)(int kind) {
+    switch (kind) {
+        case 0: return (const void*)&wn::k_bank_forward64<WN_NP>;
+        case 1: return (const void*)&wn::k_bank_backward64<WN_NP, false>;
+        case 2: return (const void*)&wn::k_bank_backward64<WN_NP, true>;
     }
     return nullptr;
 }
