@@ -274,7 +274,7 @@ typedef struct wn_routing {
     int groups_kept;    /* groups a row chooses from (equal to groups: all) */
     int renormalise;    /* 1: the weights of a row add up to scale */
     double scale;       /* of the weights */
-    double score_scale; /* of the scores, not zero; negative where a low score is a good one (sparsity costs) */
+    double score_scale; /* of the scores, 1e-100 ... 1e100 either way; negative where a low score is a good one (sparsity costs) */
 } wn_routing;
 
 /*

@@ -102,9 +102,7 @@ template <> __device__ __forceinline__ f16_bits narrow<f16_bits>(double d) {
     return {__builtin_bit_cast(unsigned short, (_Float16)round_to_odd(d))};
 }
 template <> __device__ __forceinline__ bf16_bits narrow<bf16_bits>(double d) {
-    const unsigned u = __builtin_bit_cast(unsigned, round_to_odd(d));
-    if (d != d) return {(unsigned short)((u >> 16) | 0x40u)};
-    return {(unsigned short)((u + 0x7FFFu + ((u >> 16) & 1u)) >> 16)};
+    return {__builtin_bit_cast(unsigned short, (__bf16)round_to_odd(d))};
 }
 
 // ---- 8-bit checkpoints ------------------------------------------------------------------------------------
