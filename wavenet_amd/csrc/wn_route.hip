@@ -21,6 +21,8 @@ struct RouteArgs {
     int T, F, k, groups, kept, per;   // per: filters in a group
     unsigned per_magic;      // f / per = f * per_magic >> 20, f < 1024
     int sigmoid, renorm;
+    int settle_rows;         // rows of a workgroup of the second kernel at a time, at most SETTLE_T
+    int doubts;              // values may lie closer than what the first kernel compares
     double scale, score_scale;
     const double* bias;
     int* idx;
@@ -33,6 +35,9 @@ struct RouteArgs {
 };
 
 constexpr int ROUTE_T = 256;
+#ifndef ROUTE32_WAVES
+#define ROUTE32_WAVES 2
+#endif
 constexpr unsigned long long ROUTE_LOW = WN_MAX_EXPERTS - 1;   // bits that hold a filter's number
 
 __device__ __forceinline__ double minus_inf() { return -__builtin_huge_val(); }
@@ -118,9 +123,9 @@ __device__ __forceinline__ void route_lds_order() {
     __builtin_amdgcn_wave_barrier();
 }
 
-// The shares to within ROUTE_SLACK of the true ones, from 32-bit exponentials: an argument of x has an error of |x| 2^-23 and
-// v_exp_f32, v_rcp_f32 and the sum one of 2^-22 or so each, all of it times p <= 1 with |x| p <= 0.4.
-constexpr double ROUTE_SLACK = 2e-6;
+// The shares to within ROUTE_SLACK of the true ones, from 32-bit exponentials: an argument of x is off by |x| 2^-23, v_exp_f32,
+// v_rcp_f32, the sum and the product by 2^-22 or so each, all of it times p <= 1 with |x| p <= 0.4: 0.4 * 1.2e-7 + 3 * 2.4e-7.
+constexpr double ROUTE_SLACK = 1e-6;
 __device__ __forceinline__ float rough_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504f); }
 __device__ __forceinline__ float rough_sigmoid(float s) { return __builtin_amdgcn_rcpf(1.0f + rough_exp(-s)); }
 
@@ -189,6 +194,17 @@ __device__ __forceinline__ unsigned key_lane(unsigned v, int lane) {
     else return __shfl_xor(v, M, 64);
 }
 
+// the lowest of a whole number per lane
+template <int LPR>
+__device__ __forceinline__ int row_lowest(int v, int lane) {
+    v = min(v, (int)key_lane<1>((unsigned)v, lane));
+    v = min(v, (int)key_lane<2>((unsigned)v, lane));
+    v = min(v, (int)key_lane<7>((unsigned)v, lane));
+    v = min(v, (int)key_lane<8>((unsigned)v, lane));
+    if constexpr (LPR > 16) v = min(v, (int)key_lane<16>((unsigned)v, lane));
+    if constexpr (LPR > 32) v = min(v, (int)key_lane<32>((unsigned)v, lane));
+    return v;
+}
 // a whole number per lane added up over the row
 template <int LPR>
 __device__ __forceinline__ int row_count(int v, int lane) {
@@ -285,29 +301,6 @@ __device__ __forceinline__ int filter_of(double key) {
 }
 __device__ __forceinline__ unsigned long long upper(double key) { return bits_of(key) & ~ROUTE_LOW; }
 
-// k rounds on the full values: the largest left, the lowest filter among equal ones.  c is destroyed; lane j < k of the row
-// returns the filter of round j, or -1.
-template <int LPR, int VPL>
-__device__ __forceinline__ int choose_by_rounds(double (&c)[VPL], int k, int l, int f0, int lane) {
-    int mine = -1;
-    for (int j = 0; j < k; j++) {
-        double best = c[0];
-#pragma unroll
-        for (int i = 1; i < VPL; i++) best = __builtin_fmax(best, c[i]);
-        best = row_max<LPR>(best, lane);
-        int at = VPL;
-#pragma unroll
-        for (int i = VPL - 1; i >= 0; i--) at = c[i] == best ? i : at;
-        const unsigned long long holders = (__ballot(at < VPL) >> (lane & ~(LPR - 1))) & (LPR == 64 ? ~0ull : (1ull << (LPR & 63)) - 1);
-        const int owner = __ffsll((unsigned long long)holders) - 1;
-        const int f = best == minus_inf() ? -1 : owner * VPL + __shfl(at, (lane & ~(LPR - 1)) + owner, 64);
-        if (l == j) mine = f;
-#pragma unroll
-        for (int i = 0; i < VPL; i++) c[i] = f0 + i == f ? minus_inf() : c[i];
-    }
-    return mine;
-}
-
 // ---- forward --------------------------------------------------------------------------------------------------
 
 __device__ __forceinline__ double larger_of(double a, double b) { return key_max(a, b); }
@@ -318,6 +311,39 @@ __device__ __forceinline__ float smaller_of(float a, float b) { return __builtin
 // of a >= b and v, the one in the middle
 __device__ __forceinline__ double middle_of(double a, double b, double v) { return larger_of(b, smaller_of(a, v)); }
 __device__ __forceinline__ float middle_of(float a, float b, float v) { return __builtin_amdgcn_fmed3f(a, b, v); }
+
+// The groups that are kept, as a bit mask, from the row's values in LDS: a lane per group.
+template <int LPR, class T>
+__device__ __forceinline__ unsigned long long kept_groups(T slack, const RouteArgs& A, double* crow, int l, bool& doubt) {
+    unsigned long long keep = 0;
+    double* grow = crow + A.F;
+    for (int g = l; g < A.groups; g += LPR) {
+        double first = minus_inf(), second = minus_inf();
+        for (int i = 0; i < A.per; i++) {
+            const double v = crow[g * A.per + i];
+            second = middle_of(first, second, v);
+            first = larger_of(first, v);
+        }
+        grow[g] = second > minus_inf() ? first + second : first;
+    }
+    route_lds_order();
+    for (int g = l; g < A.groups; g += LPR) {
+        const double mine = grow[g];
+        int ahead = 0, surely = 0, perhaps = 0;
+        for (int h = 0; h < A.groups; h++) {
+            const double other = grow[h];
+            ahead += other > mine || (other == mine && h < g);
+            surely += other > mine + 2 * slack;
+            perhaps += other >= mine - 2 * slack && h != g;
+        }
+        doubt |= slack > 0 && mine > minus_inf() && surely < A.kept && perhaps >= A.kept;
+        if (ahead < A.kept) keep |= 1ull << g;
+    }
+#pragma unroll
+    for (int x = 1; x < LPR; x *= 2) keep |= __shfl_xor(keep, x, 64);
+    route_lds_order();                                       // before the row's next values
+    return keep;
+}
 
 // The lane's filters that are in a group that is kept, as a bit mask; c: the row's values, each within slack / 2 of the true one.  A group that is a
 // whole number of lanes (a power of two) is reduced in registers; other sizes go through LDS, a lane per group.
@@ -350,38 +376,12 @@ __device__ __forceinline__ unsigned choose_groups(const T (&c)[VPL], T slack, co
         doubt |= slack > 0 && g < A.groups && mine > (T)minus_inf() && surely < A.kept && perhaps >= A.kept;
         return ahead < A.kept ? ~0u : 0u;
     }
-    unsigned long long keep = 0;
-    double* grow = crow + A.F;
 #pragma unroll
     for (int i = 0; i < VPL; i++) {
         if (f0 + i < A.F) crow[f0 + i] = c[i];
     }
     route_lds_order();
-    for (int g = l; g < A.groups; g += LPR) {
-        double first = minus_inf(), second = minus_inf();
-        for (int i = 0; i < A.per; i++) {
-            const double v = crow[g * A.per + i];
-            second = __builtin_fmax(second, __builtin_fmin(first, v));
-            first = __builtin_fmax(first, v);
-        }
-        grow[g] = second > minus_inf() ? first + second : first;
-    }
-    route_lds_order();
-    for (int g = l; g < A.groups; g += LPR) {
-        const double mine = grow[g];
-        int ahead = 0, surely = 0, perhaps = 0;
-        for (int h = 0; h < A.groups; h++) {
-            const double other = grow[h];
-            ahead += other > mine || (other == mine && h < g);
-            surely += other > mine + 2 * slack;
-            perhaps += other >= mine - 2 * slack && h != g;
-        }
-        doubt |= slack > 0 && mine > minus_inf() && surely < A.kept && perhaps >= A.kept;
-        if (ahead < A.kept) keep |= 1ull << g;
-    }
-#pragma unroll
-    for (int x = 1; x < LPR; x *= 2) keep |= __shfl_xor(keep, x, 64);
-    route_lds_order();                                       // before the next row's values
+    const unsigned long long keep = kept_groups<LPR, T>(slack, A, crow, l, doubt);
     unsigned own = 0;
 #pragma unroll
     for (int i = 0; i < VPL; i++) own |= ((unsigned)(keep >> (((unsigned)(f0 + i) * A.per_magic) >> 20)) & 1u) << i;
@@ -402,50 +402,6 @@ __device__ __forceinline__ void scale_row(double (&x)[VPL], const RouteArgs& A, 
     bad = row_any<LPR>(bad, lane);
     if (!A.sigmoid) m = row_max<LPR>(m, lane);
 }
-// exp(s - m) and its sum over the row
-template <int LPR, int VPL>
-__device__ __forceinline__ double exp_row(double (&e)[VPL], const double (&s)[VPL], double m, int lane) {
-    double Z = 0;
-#pragma unroll
-    for (int i = 0; i < VPL; i++) {
-        e[i] = s[i] > minus_inf() ? route_exp(s[i] - m) : 0.0;
-        Z += e[i];
-    }
-    return row_sum<LPR>(Z, lane);
-}
-
-// The whole choice in 64 bits, round by round: for the few rows that the quicker ways leave in doubt.
-template <int LPR, int VPL>
-__device__ __forceinline__ int choose_exactly(const RouteArgs& A, long long row, double* crow, int l, int f0, int lane) {
-    double s[VPL], c[VPL], m;
-    bool bad;
-    load_row<LPR, VPL>(s, A, row, f0);
-    scale_row<LPR, VPL>(s, A, m, bad, lane);
-    if (A.bias || A.kept < A.groups) {
-        if (A.sigmoid) {
-#pragma unroll
-            for (int i = 0; i < VPL; i++) c[i] = route_sigmoid(s[i]);
-        } else {
-            const double Z = exp_row<LPR, VPL>(c, s, m, lane);
-#pragma unroll
-            for (int i = 0; i < VPL; i++) c[i] /= Z;
-        }
-#pragma unroll
-        for (int i = 0; i < VPL; i++) {
-            if (A.bias) c[i] += A.bias[f0 + i < A.F ? f0 + i : A.F - 1];
-            c[i] = (s[i] > minus_inf() && c[i] > minus_inf()) ? c[i] : minus_inf();
-        }
-        if (A.kept < A.groups) {
-            bool doubt = false;
-            const unsigned keep = choose_groups<LPR, VPL>(c, 0.0, A, crow, l, f0, lane, doubt);
-#pragma unroll
-            for (int i = 0; i < VPL; i++) c[i] = (keep >> i) & 1 ? (A.bias ? c[i] : s[i]) : minus_inf();
-        }
-        return choose_by_rounds<LPR, VPL>(c, A.k, l, f0, lane);
-    }
-    return choose_by_rounds<LPR, VPL>(s, A.k, l, f0, lane);
-}
-
 // The weights of a row, one chosen filter (or -1) per lane, and what leaves.
 template <int LPR, int VPL>
 __device__ __forceinline__ void finish_row(const RouteArgs& A, long long row, int f, bool bad, bool write, int l, int f0, int lane) {
@@ -476,7 +432,10 @@ __device__ __forceinline__ void finish_row(const RouteArgs& A, long long row, in
         bool unused;
         load_row<LPR, VPL>(all, A, row, f0);
         scale_row<LPR, VPL>(all, A, m, unused, lane);
-        const double Z = exp_row<LPR, VPL>(all, all, m, lane);
+        double Z = 0;
+#pragma unroll
+        for (int i = 0; i < VPL; i++) Z += all[i] > minus_inf() ? route_exp(all[i] - m) : 0.0;
+        Z = row_sum<LPR>(Z, lane);
         if (have) w = A.scale * (route_exp(s - m) / Z);
     }
     if (bad) w = __builtin_nan("");
@@ -486,39 +445,18 @@ __device__ __forceinline__ void finish_row(const RouteArgs& A, long long row, in
     }
 }
 
-// A row that the quicker ways leave in doubt has ROUTE_DOUBT for its first index until the workgroup is through with the
-// others, and is then chosen in 64 bits: at that point this holds no registers that the loops need.
+// A row whose values lie closer than what was compared can tell has ROUTE_DOUBT for its first index, and is chosen again by
+// the next kernel (k_route_settle): in here, the rare way would cost the registers of every row and hold up the last.
 constexpr int ROUTE_DOUBT = -2;
 template <int LPR, int VPL>
-__device__ __forceinline__ void settle_doubts(const RouteArgs& A, double* crow, int sub, int l, int lane) {
-    constexpr int ROWS = ROUTE_T / LPR;
-    for (long long base = (long long)blockIdx.x * ROWS; base < A.T; base += (long long)gridDim.x * ROWS) {
-        const bool live = base + sub < A.T;
-        const long long row = live ? base + sub : A.T - 1;
-        const bool again = live && A.idx[row * A.k] == ROUTE_DOUBT;
-        if (!__any(again)) continue;
-        int f0 = l * VPL;
-        asm volatile("" : "+v"(f0));
-        const int f = choose_exactly<LPR, VPL>(A, row, crow, l, f0, lane);
-        finish_row<LPR, VPL>(A, row, f, false, again, l, f0, lane);
-    }
-}
-__device__ __forceinline__ void route_begin(const RouteArgs& A, int* any_doubt) {
-    if (A.counts && blockIdx.x == 0) {                       // added up by the next kernel
-        for (int f = threadIdx.x; f < A.F; f += ROUTE_T) A.counts[f] = 0;
-    }
-    if (threadIdx.x == 0) *any_doubt = 0;
-    __syncthreads();
-}
-// what leaves of a row, or that it is in doubt
-template <int LPR, int VPL>
-__device__ __forceinline__ void route_row(const RouteArgs& A, long long row, int f, bool bad, bool doubt, bool live, int* any_doubt, int l,
-                                          int f0, int lane) {
+__device__ __forceinline__ void route_row(const RouteArgs& A, long long row, int f, bool bad, bool doubt, bool live, int l, int f0, int lane) {
     doubt = row_any<LPR>(doubt, lane) && !bad;
     finish_row<LPR, VPL>(A, row, bad ? -1 : f, bad, live && !doubt, l, f0, lane);
-    if (doubt && live && l == 0) {
-        A.idx[row * A.k] = ROUTE_DOUBT;
-        *any_doubt = 1;
+    if (doubt && live && l == 0) A.idx[row * A.k] = ROUTE_DOUBT;
+}
+__device__ __forceinline__ void clear_counts(const RouteArgs& A) {
+    if (A.counts && blockIdx.x == 0) {                       // added up by the last kernel
+        for (int f = threadIdx.x; f < A.F; f += ROUTE_T) A.counts[f] = 0;
     }
 }
 
@@ -526,13 +464,12 @@ __device__ __forceinline__ void route_row(const RouteArgs& A, long long row, int
 template <int LPR, int VPL, int K, bool GROUPED>
 __global__ __launch_bounds__(ROUTE_T) void k_route64(RouteArgs A) {
     extern __shared__ __attribute__((aligned(16))) double route_lds[];
-    __shared__ int any_doubt;
     constexpr int ROWS = ROUTE_T / LPR;
     const int lane = threadIdx.x & 63, sub = threadIdx.x / LPR, l = threadIdx.x % LPR;
     double* crow = route_lds + sub * (A.F + A.groups + 1);   // groups only
     // 24-bit scores are compared as they are: scaled, they could need the bits that the filter's number takes
     const bool as_read = A.dtype != WN_F64;
-    route_begin(A, &any_doubt);
+    clear_counts(A);
     for (long long base = (long long)blockIdx.x * ROWS; base < A.T; base += (long long)gridDim.x * ROWS) {
         const bool live = base + sub < A.T;
         const long long row = live ? base + sub : A.T - 1;
@@ -585,40 +522,41 @@ __global__ __launch_bounds__(ROUTE_T) void k_route64(RouteArgs A) {
 #pragma unroll
             for (int i = 0; i < VPL; i++) doubt |= last > minus_inf() && c[i] != at_last && c[i] >= last - slack && c[i] <= last + slack;
         }
-        route_row<LPR, VPL>(A, row, f, bad, doubt, live, &any_doubt, l, f0, lane);
+        route_row<LPR, VPL>(A, row, f, bad, doubt, live, l, f0, lane);
     }
-    if (as_read && !GROUPED) return;
-    __syncthreads();
-    if (any_doubt) settle_doubts<LPR, VPL>(A, crow, sub, l, lane);
 }
 
 // With a bias, or 16-bit scores: 32-bit keys.  A 16-bit score stands in the upper half of its key as it is (in an order of
 // unsigned numbers).  With a bias the upper bits are the rough share plus bias, as a fraction of the range that the biases
 // leave for it.
 
-// s = scale * score as floats: finite ones within +-3e38, -inf for closed filters.  bad: a NaN or +inf among them.
+// a lane's scores as they are in memory; those beyond the filters are others of the row
 template <class S, int VPL>
-__device__ __forceinline__ void load_scaled(float (&s)[VPL], S (&v)[VPL], const RouteArgs& A, long long row, int f0, bool& bad) {
+__device__ __forceinline__ void fetch_chunk(S (&v)[VPL], const RouteArgs& A, long long row, int f0) {
     const S* p = (const S*)A.scores + row * A.rs + f0 * A.cs;
-    const float scale = (float)A.score_scale;
     const int most = A.F - 1 - f0;
-    bool odd = true;                                         // values that need a second look
-    if (A.cs == 1 && A.F == VPL * (A.F / VPL)) {             // whole chunks, or none
-        if (most < 0) p -= f0;                               // a lane beyond the filters reads what another one does
+    if (A.cs == 1 && A.F % VPL == 0) {                       // whole chunks, or none
+        if (most < 0) p -= f0;
         __builtin_memcpy(v, p, sizeof(v));                   // wide loads: the hardware takes any alignment
-        if constexpr (sizeof(S) < 8) {
-            float large = 0;
-#pragma unroll
-            for (int i = 0; i < VPL; i++) {
-                const float x = (float)widen(v[i]);
-                s[i] = x * scale;
-                large += __builtin_fabsf(s[i]);              // finite if they all are, and not too large
-            }
-            odd = !(large < 3e38f) || most < 0;
-        }
     } else {
 #pragma unroll
         for (int i = 0; i < VPL; i++) v[i] = p[(i < most ? i : most) * A.cs];
+    }
+}
+// s = scale * score as floats: finite ones within +-3e38, -inf for closed filters.  bad: a NaN or +inf among them.
+template <class S, int VPL>
+__device__ __forceinline__ void scale_chunk(float (&s)[VPL], const S (&v)[VPL], const RouteArgs& A, int f0, bool& bad) {
+    const float scale = (float)A.score_scale;
+    const int most = A.F - 1 - f0;
+    bool odd = true;                                         // values that need a second look
+    if constexpr (sizeof(S) < 8) {
+        float large = 0;
+#pragma unroll
+        for (int i = 0; i < VPL; i++) {
+            s[i] = (float)widen(v[i]) * scale;
+            large += __builtin_fabsf(s[i]);                  // finite if they all are, and not too large
+        }
+        odd = !(large < 3e38f) || most < VPL - 1;
     }
     if (!__any(odd)) return;
     const float closed = A.score_scale > 0 ? -__builtin_huge_valf() : __builtin_huge_valf();
@@ -646,9 +584,8 @@ __device__ __forceinline__ unsigned bits16(float) { return 0; }
 __device__ __forceinline__ unsigned bits16(double) { return 0; }
 
 template <class S, int LPR, int VPL, int K>
-__global__ __launch_bounds__(ROUTE_T) void k_route32(RouteArgs A) {
+__global__ __launch_bounds__(ROUTE_T, ROUTE32_WAVES) void k_route32(RouteArgs A) {
     extern __shared__ __attribute__((aligned(16))) double route_lds[];
-    __shared__ int any_doubt;
     constexpr int ROWS = ROUTE_T / LPR;
     constexpr unsigned LOW = LPR * VPL - 1;                  // bits of a key that hold the filter's number
     constexpr float STEPS = 0.99f * (float)(0xFFFFFFFFu / (LOW + 1));   // that the upper bits are cut into
@@ -674,7 +611,7 @@ __global__ __launch_bounds__(ROUTE_T) void k_route32(RouteArgs A) {
     const float steps = STEPS / range;
 #pragma unroll
     for (int i = 0; i < VPL; i++) place[i] = (bias[i] - b_min) * steps + 1.0f;
-    route_begin(A, &any_doubt);
+    clear_counts(A);
     for (long long base = (long long)blockIdx.x * ROWS; base < A.T; base += (long long)gridDim.x * ROWS) {
         const bool live = base + sub < A.T;
         const long long row = live ? base + sub : A.T - 1;
@@ -685,7 +622,8 @@ __global__ __launch_bounds__(ROUTE_T) void k_route32(RouteArgs A) {
         bool bad = false, doubt = wild;
         {
             S v[VPL];
-            load_scaled<S, VPL>(s, v, A, row, f0, bad);
+            fetch_chunk<S, VPL>(v, A, row, f0);
+            scale_chunk<S, VPL>(s, v, A, f0, bad);
             if (sizeof(S) == 2 && !biased) {
                 // by the score itself: its order is that of the shares, and equal shares of different scores are not
                 const unsigned flip = A.score_scale > 0 ? 0u : 0xFFFFu;
@@ -755,51 +693,114 @@ __global__ __launch_bounds__(ROUTE_T) void k_route32(RouteArgs A) {
             // Values within the slack of each other are not told apart by their keys.  Of the chosen ones neighbours are
             // looked at, around the last of them every value.
             const unsigned near = (unsigned)__builtin_fminf(slack * steps + STEPS * 4.8e-7f + 2.0f, STEPS) * (LOW + 1) + LOW;
-            const unsigned next = __shfl_down(mine, 1, 64);
-            bool close = l + 1 < A.k && next && mine - next <= near;
-            const unsigned lo = last > near ? last - near : 1u, hi = last < 0xFFFFFFFFu - near ? last + near : 0xFFFFFFFFu;
+            const unsigned next = __shfl_down(mine, 1, 64), lo = last > near ? last - near : 1u;
             int within = 0;
 #pragma unroll
             for (int i = 0; i < VPL; i++) within += keys[i] >= lo;
             within = row_count<LPR>(within, lane);
-            close |= last && within > A.k;
-            if (__any(close)) {
-                // Equal scores under equal biases are equal whatever the rounding, and stand in order of the filter already:
-                // look at what differs.
-                const int fs = __shfl(f, (lane - l) + A.k - 1, 64);
-                const double last_s = fs >= 0 ? score_at(A, row, fs) : 0.0, last_b = fs >= 0 ? A.bias[fs] : 0.0;
-                for (int i = 0; i < VPL; i++) {
-                    const int g = f0 + i < A.F ? f0 + i : A.F - 1;
-                    unsigned key = 0;
-#pragma unroll
-                    for (int t = 0; t < VPL; t++) key = t == i ? keys[t] : key;
-                    doubt |= fs >= 0 && key >= lo && key <= hi && (score_at(A, row, g) != last_s || A.bias[g] != last_b);
-                }
-                const double own_s = f >= 0 ? score_at(A, row, f) : 0.0, own_b = f >= 0 ? A.bias[f] : 0.0;
-                const double next_s = __shfl_down(own_s, 1, 64), next_b = __shfl_down(own_b, 1, 64);
-                doubt |= l + 1 < A.k && next && mine - next <= near && (own_s != next_s || own_b != next_b);
-            }
+            doubt |= (l + 1 < A.k && next && mine - next <= near) || (last && within > A.k);
         }
-        route_row<LPR, VPL>(A, row, f, bad, doubt, live, &any_doubt, l, f0, lane);
+        route_row<LPR, VPL>(A, row, f, bad, doubt, live, l, f0, lane);
     }
-    if (!biased && !grouped) return;
-    __syncthreads();
-    if (any_doubt) settle_doubts<LPR, VPL>(A, crow, sub, l, lane);
 }
 
-// counts[f] += entries of idx that name f: a histogram per workgroup in LDS, then one addition per filter (whole
-// numbers, so that their order does not matter).
-__global__ __launch_bounds__(1024) void k_route_counts(RouteArgs A) {
-    __shared__ int hist[WN_MAX_EXPERTS];
-    for (int f = threadIdx.x; f < A.F; f += 1024) hist[f] = 0;
-    __syncthreads();
-    const long long total = (long long)A.T * A.k;
-    for (long long i = (long long)blockIdx.x * 1024 + threadIdx.x; i < total; i += (long long)gridDim.x * 1024) {
-        const int f = A.idx_in[i];
-        if (f >= 0) atomicAdd(&hist[f], 1);
+// A marked row in 64 bits and round by round, by one wave with the values in LDS: lane j < k returns its j-th filter.  Short
+// code before quick code: rows come here one at a time, and much of what that takes is the fetching of the instructions.
+__device__ __forceinline__ int choose_exactly(const RouteArgs& A, long long row, double* crow, int lane) {
+    const bool shares = A.bias || A.kept < A.groups;
+                double m = minus_inf(), Z = 0;
+#pragma nounroll
+                for (int f = lane; f < A.F; f += 64) {
+                    const double v = A.score_scale * score_at(A, row, f);
+                    m = key_max(m, v);
+                    crow[f] = v;
+                }
+                route_lds_order();
+                if (shares) {
+                    if (!A.sigmoid) {
+                        m = row_max<64>(m, lane);
+#pragma nounroll
+                        for (int f = lane; f < A.F; f += 64) Z += crow[f] > minus_inf() ? route_exp(crow[f] - m) : 0.0;
+                        Z = row_sum<64>(Z, lane);
+                    }
+#pragma nounroll
+                    for (int f = lane; f < A.F; f += 64) {
+                        const double v0 = crow[f];
+                        double v = A.sigmoid ? route_sigmoid(v0) : route_exp(v0 - m) / Z;
+                        if (A.bias) v += A.bias[f];
+                        crow[f] = (v0 > minus_inf() && v > minus_inf()) ? v : minus_inf();
+                    }
+                    route_lds_order();
+                }
+                if (A.kept < A.groups) {
+                    bool doubt = false;
+                    const unsigned long long keep = kept_groups<64, double>(0.0, A, crow, lane, doubt);
+#pragma nounroll
+                    for (int f = lane; f < A.F; f += 64) {
+                        const bool open = (keep >> (((unsigned)f * A.per_magic) >> 20)) & 1;
+                        if (!open) crow[f] = minus_inf();
+                        else if (!A.bias && crow[f] > minus_inf()) crow[f] = A.score_scale * score_at(A, row, f);
+                    }
+                    route_lds_order();
+                }
+                int mine = -1;
+#pragma nounroll
+                for (int j = 0; j < A.k; j++) {
+                    double best = minus_inf();
+                    int at = WN_MAX_EXPERTS;
+#pragma nounroll
+                    for (int f = lane; f < A.F; f += 64) {
+                        const double v = crow[f];
+                        at = v > best ? f : at;
+                        best = key_max(best, v);
+                    }
+                    const double top = row_max<64>(best, lane);
+                    at = best == top && top > minus_inf() ? at : WN_MAX_EXPERTS;
+                    at = row_lowest<64>(at, lane);
+                    if (at < WN_MAX_EXPERTS) {
+                        if (lane == j) mine = at;
+                        if (lane == at % 64) crow[at] = minus_inf();
+                    }
+                    route_lds_order();
+                }
+    return mine;
+}
+
+// After k_route32 and k_route64: the rows that they marked (a workgroup's waves share its marked rows; equal values among
+// 16-bit scores under equal biases come here too, and may be many), and counts[f] += entries of idx that name f, by a
+// histogram per workgroup in LDS and one addition per filter (whole numbers, so that their order does not matter).
+constexpr int SETTLE_T = 1024;
+__global__ __launch_bounds__(SETTLE_T) void k_route_settle(RouteArgs A) {
+    extern __shared__ __attribute__((aligned(16))) double route_lds[];
+    __shared__ int hist[WN_MAX_EXPERTS], marked[SETTLE_T], marks;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    double* crow = route_lds + wave * (A.F + A.groups + 1);
+    for (int f = threadIdx.x; f < A.F; f += SETTLE_T) hist[f] = 0;
+    for (long long base = (long long)blockIdx.x * A.settle_rows; base < A.T; base += (long long)gridDim.x * A.settle_rows) {
+        const int rows = (int)(A.T - base < A.settle_rows ? A.T - base : A.settle_rows);
+        if (A.doubts) {
+            __syncthreads();
+            if (threadIdx.x == 0) marks = 0;
+            __syncthreads();
+            if ((int)threadIdx.x < rows && A.idx[(base + threadIdx.x) * A.k] == ROUTE_DOUBT) marked[atomicAdd(&marks, 1)] = threadIdx.x;
+            __syncthreads();
+            for (int i = wave; i < marks; i += SETTLE_T / 64) {
+                const long long row = base + marked[i];
+                const int f = choose_exactly(A, row, crow, lane);
+                finish_row<64, WN_MAX_EXPERTS / 64>(A, row, f, false, true, lane, lane * (WN_MAX_EXPERTS / 64), lane);
+            }
+        }
+        __syncthreads();
+        if (A.counts) {
+            for (int i = threadIdx.x; i < rows * A.k; i += SETTLE_T) {
+                const int f = A.idx[base * A.k + i];
+                if (f >= 0) atomicAdd(&hist[f], 1);
+            }
+        }
     }
     __syncthreads();
-    for (int f = threadIdx.x; f < A.F; f += 1024) {
+    if (!A.counts) return;
+    for (int f = threadIdx.x; f < A.F; f += SETTLE_T) {
         if (hist[f]) atomicAdd(&A.counts[f], hist[f]);
     }
 }
@@ -1001,12 +1002,15 @@ int wn_route(wn_context* ctx, const void* scores_dev, int dtype, int T, int F, l
         const RouteClass K = route_class(F, routing->k, dtype, bias_dev, routing->groups_kept < routing->groups);
         const int rows = wn::ROUTE_T / K.lpr;
         const long long grid = std::max(1LL, std::min<long long>(((long long)T + rows - 1) / rows, (long long)ctx->numCU * 4));
-        const size_t shmem = A.kept < A.groups ? (size_t)rows * (F + A.groups + 1) * sizeof(double) : 0;
-        rc = wn::launch_kernel(ctx, K.forward, (unsigned)grid, wn::ROUTE_T, shmem, A);
-        if (rc || !counts_dev || T == 0) return rc;
-        const long long entries = (long long)T * A.k;
-        const long long cgrid = std::max(1LL, std::min<long long>((entries + 16383) / 16384, 64));
-        return wn::launch_kernel(ctx, (const void*)&wn::k_route_counts, (unsigned)cgrid, 1024, 0, A);
+        A.doubts = bias_dev || A.kept < A.groups || dtype == WN_F64;
+        const size_t values = (size_t)(F + A.groups + 1) * sizeof(double);
+        rc = wn::launch_kernel(ctx, K.forward, (unsigned)grid, wn::ROUTE_T, A.kept < A.groups ? rows * values : 0, A);
+        if (rc || T == 0) return rc;
+        if (!A.doubts && !counts_dev) return WN_OK;
+        // rows spread over the chip, but no fewer than 64 to a workgroup, each of which adds to the counts
+        A.settle_rows = (int)std::min<long long>(wn::SETTLE_T, std::max<long long>(64, ((long long)T + ctx->numCU - 1) / ctx->numCU));
+        const long long sgrid = std::min<long long>(((long long)T + A.settle_rows - 1) / A.settle_rows, ctx->numCU);
+        return wn::launch_kernel(ctx, (const void*)&wn::k_route_settle, (unsigned)sgrid, wn::SETTLE_T, A.doubts ? wn::SETTLE_T / 64 * values : 0, A);
     });
 }
 
