@@ -1,7 +1,7 @@
 // Routed filter bank: wn_forward_routed, wn_backprop_routed.
 #include <algorithm>
 
-#include "wn_bank.h"
+#include "wn_bank_kernels.h"
 
 extern "C" const void* wn_kernel_bank_np2(int kind, int sc);
 extern "C" const void* wn_kernel_bank_np4(int kind, int sc);
@@ -169,9 +169,10 @@ int launch_bank(wn_context* ctx, int NP, int sc, int kind, wn::BankArgs& A) {
         const int waves = std::min(A.k, 4);
         return wn::launch_kernel(ctx, line_kernel_for(NP, kind, 1 << (A.lgR - 6)), grid_for(ctx, A.B), 64 * waves, waves * (n + 1) * sizeof(double), A);
     }
-    const int T = kSizeClasses[sc].T;
-    const size_t buffers = (A.lgC > 0 ? 4 : 3) * n, scratch = kind ? (size_t)(T / 64) * NP + 2 : 0;
-    return wn::launch_kernel(ctx, kernel_for(NP, kind != 0, sc), grid_for(ctx, A.B), T, (buffers + scratch) * sizeof(double), A);
+    // a team of threads per filter: a wave each, up to four, while a wave is enough for an example
+    const int T = kSizeClasses[sc].T, teams = T == 64 ? std::min(A.k, 4) : 1;
+    const size_t team = (size_t)wn::bank_team_doubles((int)n, A.lgC > 0, kind ? T / 64 * NP + 2 : 0);
+    return wn::launch_kernel(ctx, kernel_for(NP, kind != 0, sc), grid_for(ctx, A.B), T * teams, (n + teams * (1 + team)) * sizeof(double), A);
 }
 
 }  // namespace
