@@ -118,12 +118,32 @@ __device__ __forceinline__ int ckpt_quantise(double x, float scale) {
     const double r = __builtin_rint(x / (double)scale);
     return (int)__builtin_fmin(127.0, __builtin_fmax(-127.0, r));
 }
-// The same from inv = 1 / scale: x * inv is within 2^-45 of x / scale, so that it rounds alike unless it lies next to the
-// middle between two whole numbers, and only then is the division made.
-__device__ __forceinline__ int ckpt_quantise_fast(double x, float scale, double inv) {
-    const double t = x * inv, r = __builtin_rint(t);
-    if (__builtin_fabs(t - r) <= 0.499999 && __builtin_fabs(r) <= 127.0) return (int)r;
-    return ckpt_quantise(x, scale);                        // NaN and what does not fit come here too
+// The same, unless odd is set, from inv = ckpt_inverse(scale): x * inv is within 2^-45 of x / scale, so that it rounds alike
+// but next to the middle between two whole numbers.  Adding 1.5 * 2^52 leaves the nearest whole number in the low bits.
+// Values that are not finite are odd, too.
+__device__ __forceinline__ double ckpt_inverse(float scale) {
+    return (scale > 0.0f && scale <= 3.402823466e38f) ? 1.0 / (double)scale : 0.0;
+}
+__device__ __forceinline__ int ckpt_quantise_fast(double x, double inv, bool& odd) {
+    const double t = x * inv, s = t + 6755399441055744.0;
+    odd |= !(__builtin_fabs(t - (s - 6755399441055744.0)) <= 0.499999) || __builtin_fabs(t) > 127.4;
+    return __double2loint(s);
+}
+__device__ __forceinline__ void ckpt_quantise4(int (&b)[4], const double (&v)[4], float scale) {
+    const double inv = ckpt_inverse(scale);
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < 4; i++) b[i] = ckpt_quantise_fast(v[i], inv, odd);
+    if (__any(odd)) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) b[i] = ckpt_quantise(v[i], scale);
+    }
+}
+// larger of |a| and |b|, NaN losing: for values of which the odd ones are looked at again
+__device__ __forceinline__ double ckpt_max_quick(double a, double b) {
+    double r;
+    asm("v_max_f64 %0, |%1|, |%2|" : "=v"(r) : "v"(a), "v"(b));
+    return r;
 }
 // |x|, or a NaN for what no scale can hold; the larger of two such magnitudes, NaN winning
 __device__ __forceinline__ double ckpt_magnitude(double x) { return __builtin_fabs(x) <= 1.7976931348623157e308 ? __builtin_fabs(x) : __builtin_nan(""); }

@@ -39,58 +39,77 @@ __device__ __forceinline__ int quad_lane(int v) {   // of the quad's lane I
     return __builtin_amdgcn_update_dpp(0, v, I * 0x55, 0xF, 0xF, true);
 }
 
-__device__ __forceinline__ void bank_load64_q(double (&v)[64], const signed char* q, const float* qs, int lane) {
-    const int shift = 8 * (lane & 3);
-    const float scale = qs[lane];
+struct Bank64Q {
     int d[16];
+    float scale;           // of column `lane`
+};
+__device__ __forceinline__ void bank_fetch64_q(Bank64Q& c, const signed char* q, const float* qs, int lane) {
     const int* p = reinterpret_cast<const int*>(q);
-    asm volatile("" : "+s"(p));                            // read again where it is read again, not held in registers
+    asm volatile("" : "+s"(p), "+s"(qs));
+    c.scale = qs[lane];
     p += 16 * (lane & 3) + (lane >> 2);
 #pragma unroll
-    for (int m = 0; m < 16; m++) d[m] = p[64 * m];
+    for (int m = 0; m < 16; m++) c.d[m] = p[64 * m];
+}
+__device__ __forceinline__ void bank_values64_q(double (&v)[64], const Bank64Q& c, int lane) {
+    const int shift = 24 - 8 * (lane & 3);
 #pragma unroll
     for (int m = 0; m < 16; m++) {
-        const int b[4] = {quad_lane<0>(d[m]), quad_lane<1>(d[m]), quad_lane<2>(d[m]), quad_lane<3>(d[m])};
+        const int b[4] = {quad_lane<0>(c.d[m]), quad_lane<1>(c.d[m]), quad_lane<2>(c.d[m]), quad_lane<3>(c.d[m])};
 #pragma unroll
         for (int t = 0; t < 4; t++) {
-            const float sc = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, scale), 4 * m + t));
+            const float sc = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, c.scale), 4 * m + t));
             // a byte times a float scale is exact in a double
-            v[4 * m + t] = (double)(__builtin_bit_cast(int, (unsigned)(b[t] >> shift) << 24) >> 24) * (double)sc;
+            v[4 * m + t] = (double)((b[t] << shift) >> 24) * (double)sc;
         }
     }
 }
 
-// Largest magnitude of every column: lane c returns that of column c.  As wave_scatter_sums (wn_device.h): on lane bit t a
-// lane keeps the half of its columns whose number has that bit equal to its own.
-template <int CNT>
-__device__ __forceinline__ void bank_column_max(double (&m)[32], int lane) {
-    if constexpr (CNT > 1) {
-        constexpr int H = CNT / 2;
-        const bool up = (lane & H) != 0;
-#pragma unroll
-        for (int i = 0; i < H; i++) {
-            const double keep = up ? m[i + H] : m[i], send = up ? m[i] : m[i + H];
-            m[i] = ckpt_max(keep, xlane<H>(send, lane));
-        }
-        bank_column_max<H>(m, lane);
-    }
+// Largest magnitude of every column: lane c returns that of column c.  On lane bit t a lane keeps the half of its columns
+// whose number has that bit equal to its own.  EXACT: NaN wins; else it may be lost.  The two wide exchanges are the
+// hardware's swaps of half waves and half of their halves, which leave both operands where the maximum wants them.
+template <bool EXACT>
+__device__ __forceinline__ double bank_larger(double a, double b) {
+    if constexpr (EXACT) return ckpt_max(ckpt_magnitude(a), ckpt_magnitude(b));
+    else return ckpt_max_quick(a, b);
 }
+template <int H, bool EXACT>
+__device__ __forceinline__ void bank_column_max(double (&m)[32], int lane) {
+    const bool up = (lane & H) != 0;
+#pragma unroll
+    for (int i = 0; i < H; i++) {
+        const double keep = up ? m[i + H] : m[i], send = up ? m[i] : m[i + H];
+        m[i] = bank_larger<EXACT>(keep, xlane<H>(send, lane));
+    }
+    if constexpr (H > 1) bank_column_max<H / 2, EXACT>(m, lane);
+}
+template <int W, bool EXACT>
+__device__ __forceinline__ double bank_swap_max(double a, double b) {
+    auto swap = [](unsigned x, unsigned y) {
+        if constexpr (W == 32) return __builtin_amdgcn_permlane32_swap(x, y, false, false);
+        else return __builtin_amdgcn_permlane16_swap(x, y, false, false);
+    };
+    const auto lo = swap((unsigned)__double2loint(a), (unsigned)__double2loint(b));
+    const auto hi = swap((unsigned)__double2hiint(a), (unsigned)__double2hiint(b));
+    return bank_larger<EXACT>(__hiloint2double((int)hi[0], (int)lo[0]), __hiloint2double((int)hi[1], (int)lo[1]));
+}
+template <bool EXACT>
 __device__ __forceinline__ double bank_max64(const double (&v)[64], int lane) {
     double m[32];
-    const bool up = (lane & 32) != 0;
 #pragma unroll
-    for (int i = 0; i < 32; i++) {
-        const double lo = ckpt_magnitude(v[i]), hi = ckpt_magnitude(v[i + 32]);
-        m[i] = ckpt_max(up ? hi : lo, xlane<32>(up ? lo : hi, lane));
-    }
-    bank_column_max<32>(m, lane);
+    for (int i = 0; i < 32; i++) m[i] = bank_swap_max<32, EXACT>(v[i], v[i + 32]);
+#pragma unroll
+    for (int i = 0; i < 16; i++) m[i] = bank_swap_max<16, EXACT>(m[i], m[i + 16]);
+    bank_column_max<8, EXACT>(m, lane);
     return m[0];
 }
 
 // Columns 4 m ... 4 m + 3 for the groups m = first, first + step, ... (the registers are indexed at compile time)
-__device__ __forceinline__ void bank_keep64(const double (&v)[64], signed char* q, float* qs, int first, int step, int lane) {
-    const float scale = ckpt_scale(bank_max64(v, lane));
-    const double inv = 1.0 / (double)scale;
+template <bool EXACT>
+__device__ __forceinline__ bool bank_keep64(const double (&v)[64], signed char* q, float* qs, int first, int step, int lane) {
+    const float scale = ckpt_scale(bank_max64<EXACT>(v, lane));
+    const double inv = ckpt_inverse(scale);
+    bool odd = false;
     if (first == 0) qs[lane] = scale;
     int* out = reinterpret_cast<int*>(q) + 16 * (lane & 3) + (lane >> 2);
     const int shift = 8 * (lane & 3);
@@ -102,14 +121,20 @@ __device__ __forceinline__ void bank_keep64(const double (&v)[64], signed char* 
         unsigned own = 0;
 #pragma unroll
         for (int t = 0; t < 4; t++) {
-            const float sc = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, scale), 4 * m + t));
-            const double in = __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(inv), 4 * m + t),
-                                               __builtin_amdgcn_readlane(__double2loint(inv), 4 * m + t));
-            own |= (unsigned)(ckpt_quantise_fast(v[4 * m + t], sc, in) & 0xFF) << (8 * t);
+            int b;
+            if constexpr (EXACT) {
+                b = ckpt_quantise(v[4 * m + t], __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, scale), 4 * m + t)));
+            } else {
+                b = ckpt_quantise_fast(v[4 * m + t],
+                                       __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(inv), 4 * m + t),
+                                                        __builtin_amdgcn_readlane(__double2loint(inv), 4 * m + t)), odd);
+            }
+            own |= (unsigned)(b & 0xFF) << (8 * t);
         }
         const int s0 = quad_lane<0>((int)own), s1 = quad_lane<1>((int)own), s2 = quad_lane<2>((int)own), s3 = quad_lane<3>((int)own);
         out[64 * m] = ((s0 >> shift) & 0xFF) | (((s1 >> shift) & 0xFF) << 8) | (((s2 >> shift) & 0xFF) << 16) | (((s3 >> shift) & 0xFF) << 24);
     }
+    return odd;
 }
 
 // Columns wave, wave + waves, ... of the sum of the waves' tiles times their weights: to memory, or on top of what an
@@ -150,10 +175,13 @@ __device__ __forceinline__ void bank_pin(double (&gL)[NP], double (&gH)[NP]) {
 
 // ---- kernels ----------------------------------------------------------------------------------------------
 
+// The next example's rows are on their way while this one is worked on (the registers are there, at one wave per SIMD).
 template <int NP>
 __global__ __launch_bounds__(256, 1) void k_bank_forward64(BankArgs A) {
     extern __shared__ __attribute__((aligned(16))) double smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+    double x[64];
+    if (blockIdx.x < A.B) w64_load_rows(x, A.X + (size_t)blockIdx.x * 4096, lane);
     for (int e = blockIdx.x; e < A.B; e += gridDim.x) {
         const size_t off = (size_t)e * 4096;
         unsigned tile_off = (unsigned)wave * W64_TILE;
@@ -166,19 +194,23 @@ __global__ __launch_bounds__(256, 1) void k_bank_forward64(BankArgs A) {
             int f = 0;
             double wgt = 0;
             const bool named = j < A.k && bank_entry(A, e, j, f, wgt);
-            const bool keep = j0 == 0 && A.q_out;
-            if (named || keep) w64_load_rows(v, A.X + off, lane);
-            if (keep) bank_keep64(v, A.q_out + off, A.qs_out + (size_t)e * 64, wave, waves, lane);
+            if (j0 == 0 && A.q_out) {
+                float* qs = A.qs_out + (size_t)e * 64;
+                const bool odd = bank_keep64<false>(x, A.q_out + off, qs, wave, waves, lane);
+                if (__any(odd)) bank_keep64<true>(x, A.q_out + off, qs, wave, waves, lane);
+            }
             if (named) {
                 double a[NP], b[NP];
                 const double sg = bank_taps64<NP>(A.filters + (size_t)f * A.N, A.N, a, b);
-                w64_fwd_levels<NP, 5, true>(v, p, w, trow, a, b);
+                w64_fwd_levels<NP, 5, true>(x, p, w, trow, a, b);
+                if (j0 + waves >= A.k && e + gridDim.x < A.B) w64_load_rows(x, A.X + off + (size_t)gridDim.x * 4096, lane);
                 w64_read_transposed(w, tile, lane);
                 w64_fwd_levels<NP, 5, false>(w, p, v, trow, a, b);   // v = Y(:, lane)
                 if (BANK_B_FROM_A<NP> && sg < 0) bank_signs64(v, sg, lane);
 #pragma unroll
                 for (int r = 0; r < 64; r++) trow[r] = v[r];
             } else {
+                if (j0 + waves >= A.k && e + gridDim.x < A.B) w64_load_rows(x, A.X + off + (size_t)gridDim.x * 4096, lane);
 #pragma unroll
                 for (int r = 0; r < 64; r++) trow[r] = 0.0;           // times the weight: a NaN where that says there is no answer
             }
@@ -205,20 +237,22 @@ __global__ __launch_bounds__(256, 1) void k_bank_backward64(BankArgs A) {
             const int j = j0 + wave;
             const size_t at = (size_t)e * A.k + j;
             int f = 0;
-            double wgt = 0;
+            double wgt = 0, d[64];
+            Bank64Q c;
+            w64_load_rows(d, A.D + off, lane);             // on their way before it is known which filter to fetch
+            if constexpr (FROM_Q) bank_fetch64_q(c, A.q + off, A.qs + (size_t)e * 64, lane);
             if (j < A.k && bank_entry(A, e, j, f, wgt)) {
-                double a[NP], b[NP], v[64], w[64], d[64];
+                double a[NP], b[NP], w[64];
                 const double sg = bank_taps64<NP>(A.filters + (size_t)f * A.N, A.N, a, b);
-                w64_load_rows(d, A.D + off, lane);
                 w64_transpose(d, tile, lane);                          // d[r] = errors on Y(r, lane)
                 if (BANK_B_FROM_A<NP> && sg < 0) bank_signs64(d, sg, lane);
-                if constexpr (FROM_Q) bank_load64_q(v, A.q + off, A.qs + (size_t)e * 64, lane);
-                else w64_load_rows(v, A.X + off, lane);
                 {
-                    double p[64];
+                    double v[64], p[64];
+                    if constexpr (FROM_Q) bank_values64_q(v, c, lane);
+                    else w64_load_rows(v, A.X + off, lane);
                     w64_fwd_levels<NP, 5, true>(v, p, w, trow, a, b);
-                        w64_read_transposed(w, tile, lane);                // w[r] = Y1(r, lane)
-                        w64_pyramid_to_tile<NP, 5>(w, p, trow, a);
+                    w64_read_transposed(w, tile, lane);                // w[r] = Y1(r, lane)
+                    w64_pyramid_to_tile<NP, 5>(w, p, trow, a);
                 }
                 double gL[NP], gH[NP];
 #pragma unroll
@@ -226,8 +260,12 @@ __global__ __launch_bounds__(256, 1) void k_bank_backward64(BankArgs A) {
                 w64_bwd_levels<NP, 0, W64_TOP_TILE, true>(d, w, trow, a, b, gL, gH);   // columns
                 bank_pin<NP>(gL, gH);
                 w64_read_transposed(d, tile, lane);                    // d[c] = errors on Y1(lane, c)
-                if constexpr (FROM_Q) bank_load64_q(w, A.q + off, A.qs + (size_t)e * 64, lane);
-                else w64_load_rows(w, A.X + off, lane);
+                if constexpr (FROM_Q) {
+                    bank_fetch64_q(c, A.q + off, A.qs + (size_t)e * 64, lane);      // again, and not held in registers until here
+                    bank_values64_q(w, c, lane);
+                } else {
+                    w64_load_rows(w, A.X + off, lane);
+                }
                 {
                     double p[64];
                     w64_pyramid_to_tile<NP, 5>(w, p, trow, a);
@@ -236,7 +274,7 @@ __global__ __launch_bounds__(256, 1) void k_bank_backward64(BankArgs A) {
                 bank_pin<NP>(gL, gH);
                 double dot = 0;
 #pragma unroll
-                for (int c = 0; c < 64; c++) dot = __builtin_fma(trow[c], w[c], dot);
+                for (int i = 0; i < 64; i++) dot = __builtin_fma(trow[i], w[i], dot);
                 dot = wave_allsum(dot, lane);                          // <D, F X> = <F^T D, X>
                 if (A.dw && lane == 0) A.dw[at] = dot;
                 const double g = bank_gradient<NP, 64>(gL, gH, A.N, nullptr, lane, sg);
@@ -247,7 +285,7 @@ __global__ __launch_bounds__(256, 1) void k_bank_backward64(BankArgs A) {
                     if (A.dw && lane == 0) A.dw[at] = 0.0;
                 }
 #pragma unroll
-                for (int c = 0; c < 64; c++) trow[c] = 0.0;
+                for (int i = 0; i < 64; i++) trow[i] = 0.0;
             }
             if (lane == 0) smem[waves * W64_TILE + wave] = wgt;
             __syncthreads();

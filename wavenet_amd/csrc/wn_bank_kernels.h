@@ -72,9 +72,11 @@ __device__ __forceinline__ void bank_keep(const double* x, int n, signed char* q
         m = ckpt_max(m, xlane<4>(m, lane));
         m = ckpt_max(m, xlane<8>(m, lane));
         const float scale = ckpt_scale(m);
+        int b[4];
+        ckpt_quantise4(b, v, scale);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            if (at + i < n) q[at + i] = (signed char)ckpt_quantise(v[i], scale);
+            if (at + i < n) q[at + i] = (signed char)b[i];
         }
         if ((tid & 15) == 0 && at < n) qs[at / CKPT_BLOCK] = scale;
     }

@@ -44,10 +44,15 @@ __device__ __forceinline__ void bank_keep_line(const double (&x)[M], signed char
     if constexpr (M <= 4) m = ckpt_max(m, xlane<8>(m, lane));
     if constexpr (M <= 2) m = ckpt_max(m, xlane<16>(m, lane));
     const float scale = ckpt_scale(m);
-    const double inv = 1.0 / (double)scale;
+    const double inv = ckpt_inverse(scale);
     signed char b[M];
+    bool odd = false;
 #pragma unroll
-    for (int i = 0; i < M; i++) b[i] = (signed char)ckpt_quantise_fast(x[i], scale, inv);
+    for (int i = 0; i < M; i++) b[i] = (signed char)ckpt_quantise_fast(x[i], inv, odd);
+    if (__any(odd)) {
+#pragma unroll
+        for (int i = 0; i < M; i++) b[i] = (signed char)ckpt_quantise(x[i], scale);
+    }
     __builtin_memcpy(q + M * lane, b, M);
     if (M * lane % CKPT_BLOCK == 0) qs[M * lane / CKPT_BLOCK] = scale;
 }
