@@ -4,6 +4,7 @@ Device buffers are passed as integer addresses (e.g. torch.Tensor.data_ptr()); t
 used by callers for device memory and streams, never for the arithmetic.
 """
 import ctypes as C
+import functools
 import os
 
 import numpy as np
@@ -147,8 +148,14 @@ def _hd(a):
 _TYPE_CODES = {"float64": WN_F64, "float32": WN_F32, "float16": WN_F16, "bfloat16": WN_BF16}
 
 
+_type_names = {}
+
+
 def _type_name(x):
-    return str(x.dtype).rsplit(".", 1)[-1]
+    name = _type_names.get(x.dtype)
+    if name is None:
+        name = _type_names[x.dtype] = str(x.dtype).rsplit(".", 1)[-1]
+    return name
 
 
 def _dtype_code(x, dtype):
@@ -284,27 +291,28 @@ class Context:
                                                  f.shape[1], _addr(S)))
 
     # routed filter bank ---------------------------------------------------------------------------
-    def _buffer(self, name, x, count, *types, span=None):
+    def _buffer(self, name, x, count, wanted=None, span=None):
         """Address of an argument.  A tensor has to lie on the context's GPU, hold `count` elements (or with `span` reach
-        that far from its first) of one of the types, densely; an address is taken as it is."""
+        that far from its first) of the type, densely; an address is taken as it is."""
         if x is None or isinstance(x, int):
             return x
-        if not x.is_cuda or x.device.index != self.device:
+        if not x.is_cuda or x.get_device() != self.device:
             raise ValueError(f"{name} is on {x.device}, the context on GPU {self.device}")
-        if types and _type_name(x) not in types:
-            raise ValueError(f"{name} holds {_type_name(x)}, not {' or '.join(types)}")
+        if wanted is not None and _type_name(x) != wanted:
+            raise ValueError(f"{name} holds {_type_name(x)}, not {wanted}")
         if span is None:
             if not x.is_contiguous():
                 raise ValueError(f"{name} is not contiguous")
             if x.numel() < count:
                 raise ValueError(f"{name} holds {x.numel()} elements, {count} are needed")
-        else:
+        elif not x.is_contiguous() or x.numel() < span:
             held = x.untyped_storage().nbytes() // x.element_size() - x.storage_offset()
             if held < span:
                 raise ValueError(f"{name} ends {held} elements after its start, {span} are needed")
         return x.data_ptr()
 
     @staticmethod
+    @functools.lru_cache(maxsize=64)
     def _routing(k, score, groups, groups_kept, renormalise, scale, score_scale):
         code = {"softmax": WN_SCORE_SOFTMAX, "sigmoid": WN_SCORE_SIGMOID}.get(score, score)
         if not isinstance(code, int):

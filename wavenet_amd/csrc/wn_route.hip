@@ -22,6 +22,7 @@ struct RouteArgs {
     unsigned per_magic;      // f / per = f * per_magic >> 20, f < 1024
     int sigmoid, renorm;
     int settle_rows;         // rows of a workgroup of the second kernel at a time, at most SETTLE_T
+    int count_here;          // the first kernel counts, there is no second one
     int doubts;              // values may lie closer than what the first kernel compares
     double scale, score_scale;
     const double* bias;
@@ -459,6 +460,15 @@ __device__ __forceinline__ void clear_counts(const RouteArgs& A) {
         for (int f = threadIdx.x; f < A.F; f += ROUTE_T) A.counts[f] = 0;
     }
 }
+// A workgroup that is alone, with no row left in doubt, counts what it wrote itself.
+__device__ __forceinline__ void count_here(const RouteArgs& A) {
+    if (!A.count_here) return;
+    __syncthreads();                                         // the zeros and the indices are written
+    for (int i = threadIdx.x; i < A.T * A.k; i += ROUTE_T) {
+        const int f = A.idx[i];
+        if (f >= 0) atomicAdd(&A.counts[f], 1);
+    }
+}
 
 // 32- and 64-bit scores without a bias: 64-bit keys.  GROUPED: the groups are chosen by rough shares.
 template <int LPR, int VPL, int K, bool GROUPED>
@@ -524,6 +534,7 @@ __global__ __launch_bounds__(ROUTE_T) void k_route64(RouteArgs A) {
         }
         route_row<LPR, VPL>(A, row, f, bad, doubt, live, l, f0, lane);
     }
+    count_here(A);
 }
 
 // With a bias, or 16-bit scores: 32-bit keys.  A 16-bit score stands in the upper half of its key as it is (in an order of
@@ -702,6 +713,7 @@ __global__ __launch_bounds__(ROUTE_T, ROUTE32_WAVES) void k_route32(RouteArgs A)
         }
         route_row<LPR, VPL>(A, row, f, bad, doubt, live, l, f0, lane);
     }
+    count_here(A);
 }
 
 // A marked row in 64 bits and round by round, by one wave with the values in LDS: lane j < k returns its j-th filter.  Short
@@ -1003,12 +1015,13 @@ int wn_route(wn_context* ctx, const void* scores_dev, int dtype, int T, int F, l
         const int rows = wn::ROUTE_T / K.lpr;
         const long long grid = std::max(1LL, std::min<long long>(((long long)T + rows - 1) / rows, (long long)ctx->numCU * 4));
         A.doubts = bias_dev || A.kept < A.groups || dtype == WN_F64;
+        A.count_here = counts_dev && grid == 1 && !A.doubts;
         const size_t values = (size_t)(F + A.groups + 1) * sizeof(double);
         rc = wn::launch_kernel(ctx, K.forward, (unsigned)grid, wn::ROUTE_T, A.kept < A.groups ? rows * values : 0, A);
         if (rc || T == 0) return rc;
-        if (!A.doubts && !counts_dev) return WN_OK;
-        // rows spread over the chip, but no fewer than 64 to a workgroup, each of which adds to the counts
-        A.settle_rows = (int)std::min<long long>(wn::SETTLE_T, std::max<long long>(64, ((long long)T + ctx->numCU - 1) / ctx->numCU));
+        if (!A.doubts && (!counts_dev || A.count_here)) return WN_OK;
+        // rows spread over the chip, but no fewer than 256 to a workgroup, each of which adds to the counts
+        A.settle_rows = (int)std::min<long long>(wn::SETTLE_T, std::max<long long>(256, ((long long)T + ctx->numCU - 1) / ctx->numCU));
         const long long sgrid = std::min<long long>(((long long)T + A.settle_rows - 1) / A.settle_rows, ctx->numCU);
         return wn::launch_kernel(ctx, (const void*)&wn::k_route_settle, (unsigned)sgrid, wn::SETTLE_T, A.doubts ? wn::SETTLE_T / 64 * values : 0, A);
     });
