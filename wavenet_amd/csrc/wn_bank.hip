@@ -163,8 +163,8 @@ int launch_bank(wn_context* ctx, int NP, int sc, int kind, wn::BankArgs& A) {
     if (ctx->wave64 && A.lgR == 6 && A.lgC == 6) {
         // a workgroup per example, a wave per filter, up to the four waves whose tiles fit a CU
         const int waves = std::min(A.k, 4);
-        // forward: as many workgroups as are on the chip at a time, each fetching its next example early
-        const unsigned grid = kind == 0 ? (unsigned)std::min(A.B, ctx->numCU * (4 / waves)) : grid_for(ctx, A.B);
+        // as many workgroups as are on the chip at a time, each fetching its next example early
+        const unsigned grid = (unsigned)std::min(A.B, ctx->numCU * (4 / waves));
         return wn::launch_kernel(ctx, kernel64_for(NP, kind), grid, 64 * waves, waves * wn::BANK_TILE, A);
     }
     if (ctx->wave64 && A.lgC == 0 && A.lgR >= 7 && A.lgR <= 10) {

@@ -174,6 +174,7 @@ __device__ __forceinline__ void bank_pin(double (&gL)[NP], double (&gH)[NP]) {
 }
 
 // ---- kernels ----------------------------------------------------------------------------------------------
+// (An example is 32 KiB: e + gridDim.x stays far below 2^31.)
 
 // The next example's rows are on their way while this one is worked on (the registers are there, at one wave per SIMD).
 template <int NP>
@@ -227,6 +228,13 @@ __global__ __launch_bounds__(256, 1) void k_bank_backward64(BankArgs A) {
     extern __shared__ __attribute__((aligned(16))) double smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
     const int dpad = (NP - A.N) / 2;
+    double d[64];
+    Bank64Q c;
+    const auto fetch = [&](int e) {
+        w64_load_rows(d, A.D + (size_t)e * 4096, lane);
+        if constexpr (FROM_Q) bank_fetch64_q(c, A.q + (size_t)e * 4096, A.qs + (size_t)e * 64, lane);
+    };
+    if (blockIdx.x < A.B) fetch(blockIdx.x);
     for (int e = blockIdx.x; e < A.B; e += gridDim.x) {
         const size_t off = (size_t)e * 4096;
         unsigned tile_off = (unsigned)wave * W64_TILE;
@@ -237,10 +245,7 @@ __global__ __launch_bounds__(256, 1) void k_bank_backward64(BankArgs A) {
             const int j = j0 + wave;
             const size_t at = (size_t)e * A.k + j;
             int f = 0;
-            double wgt = 0, d[64];
-            Bank64Q c;
-            w64_load_rows(d, A.D + off, lane);             // on their way before it is known which filter to fetch
-            if constexpr (FROM_Q) bank_fetch64_q(c, A.q + off, A.qs + (size_t)e * 64, lane);
+            double wgt = 0;
             if (j < A.k && bank_entry(A, e, j, f, wgt)) {
                 double a[NP], b[NP], w[64];
                 const double sg = bank_taps64<NP>(A.filters + (size_t)f * A.N, A.N, a, b);
@@ -288,6 +293,10 @@ __global__ __launch_bounds__(256, 1) void k_bank_backward64(BankArgs A) {
                 for (int i = 0; i < 64; i++) trow[i] = 0.0;
             }
             if (lane == 0) smem[waves * W64_TILE + wave] = wgt;
+            {   // the errors that come next are on their way while the results are put together
+                const int next = j0 + waves < A.k ? e : e + (int)gridDim.x;
+                if (next < A.B) fetch(next);
+            }
             __syncthreads();
             if (A.dX) bank_join64<true>(smem, A.dX + off, j0 > 0, wave, waves, lane);
             __syncthreads();

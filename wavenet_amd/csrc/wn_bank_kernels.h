@@ -22,7 +22,7 @@ __device__ __forceinline__ void bank_taps(const double* taps, int N, double (&a)
 }
 
 // Filter and weight of entry (e, j); false where the index names no filter.
-__device__ __forceinline__ bool bank_entry(const BankArgs& A, int e, int j, int& f, double& w) {
+__device__ __forceinline__ bool bank_entry(const BankArgs& A, unsigned e, int j, int& f, double& w) {
     const size_t at = (size_t)e * A.k + j;
     f = __builtin_amdgcn_readfirstlane(A.idx ? A.idx[at] : 0);
     w = A.w ? A.w[at] : 1.0;
@@ -119,7 +119,7 @@ __global__ __launch_bounds__(T == 64 ? 256 : T) void k_bank_forward(BankArgs A) 
     double* bufY = weights + G.teams + G.team * stride;
     double* bufP = bufY + n;
     double* bufY1 = rows ? bufP + n : bufX;
-    for (int e = blockIdx.x; e < A.B; e += gridDim.x) {
+    for (unsigned e = blockIdx.x; e < (unsigned)A.B; e += gridDim.x) {
         const size_t off = (size_t)e * n;
         for (int i = threadIdx.x; i < n; i += blockDim.x) bufX[i] = A.X[off + i];
         __syncthreads();
@@ -159,7 +159,7 @@ __global__ __launch_bounds__(T == 64 ? 256 : T) void k_bank_backward(BankArgs A)
     double* bufY1 = rows ? bufP + n : bufX;
     double* red = bufD + (rows ? 3 : 2) * n;
     const int d = (NP - A.N) / 2;
-    for (int e = blockIdx.x; e < A.B; e += gridDim.x) {
+    for (unsigned e = blockIdx.x; e < (unsigned)A.B; e += gridDim.x) {
         const size_t off = (size_t)e * n;
         for (int i = threadIdx.x; i < n; i += blockDim.x)
             bufX[i] = A.X ? A.X[off + i] : (double)A.q[off + i] * (double)A.qs[(size_t)e * nb + i / CKPT_BLOCK];

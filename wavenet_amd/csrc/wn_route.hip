@@ -36,9 +36,6 @@ struct RouteArgs {
 };
 
 constexpr int ROUTE_T = 256;
-#ifndef ROUTE32_WAVES
-#define ROUTE32_WAVES 2
-#endif
 constexpr unsigned long long ROUTE_LOW = WN_MAX_EXPERTS - 1;   // bits that hold a filter's number
 
 __device__ __forceinline__ double minus_inf() { return -__builtin_huge_val(); }
@@ -368,11 +365,18 @@ __device__ __forceinline__ unsigned choose_groups(const T (&c)[VPL], T slack, co
         const T mine = second > (T)minus_inf() ? first + second : first;
         const int g = l / lanes;
         int ahead = 0, surely = 0, perhaps = 0;
-        for (int h = 0; h < A.groups; h++) {
-            const T other = __shfl(mine, (lane - l) + h * lanes, 64);
-            ahead += other > mine || (other == mine && h < g);
-            surely += other > mine + 2 * slack;
-            perhaps += other >= mine - 2 * slack && h != g;
+        for (int h0 = 0; h0 < A.groups; h0 += 4) {           // four at a time on their way
+            T other[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) other[i] = __shfl(mine, (lane - l) + ((h0 + i) * lanes & (LPR - 1)), 64);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int h = h0 + i;
+                const bool there = h < A.groups;
+                ahead += there && (other[i] > mine || (other[i] == mine && h < g));
+                surely += there && other[i] > mine + 2 * slack;
+                perhaps += there && other[i] >= mine - 2 * slack && h != g;
+            }
         }
         doubt |= slack > 0 && g < A.groups && mine > (T)minus_inf() && surely < A.kept && perhaps >= A.kept;
         return ahead < A.kept ? ~0u : 0u;
@@ -594,8 +598,10 @@ __device__ __forceinline__ unsigned bits16(bf16_bits v) { return v.v; }
 __device__ __forceinline__ unsigned bits16(float) { return 0; }
 __device__ __forceinline__ unsigned bits16(double) { return 0; }
 
+// Three waves per SIMD and as many workgroups as that makes: 65536 x 256 bf16 scores with bias and groups 72 us; two waves
+// 75, one 94, four (with spills) 113.
 template <class S, int LPR, int VPL, int K>
-__global__ __launch_bounds__(ROUTE_T, ROUTE32_WAVES) void k_route32(RouteArgs A) {
+__global__ __launch_bounds__(ROUTE_T, 3) void k_route32(RouteArgs A) {
     extern __shared__ __attribute__((aligned(16))) double route_lds[];
     constexpr int ROWS = ROUTE_T / LPR;
     constexpr unsigned LOW = LPR * VPL - 1;                  // bits of a key that hold the filter's number
@@ -819,13 +825,33 @@ __global__ __launch_bounds__(SETTLE_T) void k_route_settle(RouteArgs A) {
 
 // ---- backward -------------------------------------------------------------------------------------------------
 
+// Rounding twice, to a float and then to bf16, differs from rounding once only where the float is in the middle between two
+// of the shorter type: one chunk in some thousand, which is then rounded the long way.
 template <class S, int VPL>
+__device__ __forceinline__ void narrow_chunk(S (&v)[VPL], const double (&ds)[VPL]) {
+#pragma unroll
+    for (int i = 0; i < VPL; i++) v[i] = narrow<S>(ds[i]);
+}
+template <int VPL>
+__device__ __forceinline__ void narrow_chunk(bf16_bits (&v)[VPL], const double (&ds)[VPL]) {
+    bool middle = false;
+#pragma unroll
+    for (int i = 0; i < VPL; i++) {
+        const float f = (float)ds[i];
+        middle |= (__builtin_bit_cast(unsigned, f) & 0xFFFFu) == 0x8000u;
+        v[i] = {__builtin_bit_cast(unsigned short, (__bf16)f)};
+    }
+    if (__any(middle)) {
+#pragma unroll
+        for (int i = 0; i < VPL; i++) v[i] = narrow<bf16_bits>(ds[i]);
+    }
+}
+template <class S, int LPR, int VPL>
 __device__ __forceinline__ void store_chunk(const double (&ds)[VPL], const RouteArgs& A, long long row, int f0) {
     S* p = (S*)A.dscores + row * A.rs + f0 * A.cs;
     S v[VPL];
-#pragma unroll
-    for (int i = 0; i < VPL; i++) v[i] = narrow<S>(A.score_scale * ds[i]);
-    if (A.cs == 1 && f0 + VPL <= A.F) {
+    narrow_chunk(v, ds);
+    if (A.cs == 1 && A.F == LPR * VPL) {
         __builtin_memcpy(p, v, sizeof(v));
     } else {
 #pragma unroll
@@ -836,8 +862,9 @@ __device__ __forceinline__ void store_chunk(const double (&ds)[VPL], const Route
 }
 
 // What the chosen filters get on their own reaches the lanes that hold them through a row of LDS that is zero otherwise.
+// Three waves per SIMD: 65536 x 256 bf16, full softmax, 45 us; two 56, four (with spills) 51.
 template <int LPR, int VPL>
-__global__ __launch_bounds__(ROUTE_T) void k_route_backward(RouteArgs A) {
+__global__ __launch_bounds__(ROUTE_T, 3) void k_route_backward(RouteArgs A) {
     constexpr int ROWS = ROUTE_T / LPR;
     __shared__ __attribute__((aligned(16))) double own[ROWS][LPR * VPL];
     const int lane = threadIdx.x & 63, sub = threadIdx.x / LPR, l = threadIdx.x % LPR, f0 = l * VPL;
@@ -874,34 +901,43 @@ __global__ __launch_bounds__(ROUTE_T) void k_route_backward(RouteArgs A) {
 #pragma unroll
             for (int i = 0; i < VPL; i++) {
                 ds[i] *= A.score_scale;
-                m = __builtin_fmax(m, ds[i]);
+                m = key_max(m, ds[i]);
             }
             m = row_max<LPR>(m, lane);
             bool bad = false;
 #pragma unroll
             for (int i = 0; i < VPL; i++) {
                 bad |= !(ds[i] <= 1.7976931348623157e308);
-                ds[i] = ds[i] == minus_inf() ? 0.0 : exp(ds[i] - m);
+                ds[i] = route_exp(ds[i] - m);                // (-inf: 0, and so is -inf - -inf)
                 Z += ds[i];
             }
             Z = row_sum<LPR>(Z, lane);
             if (row_any<LPR>(bad, lane)) Z = __builtin_nan("");
             const double p = (have && s != minus_inf()) ? exp(s - m) / Z : 0.0;
             d = have ? g * p : 0.0;
-            // a row without a chosen filter has no gradient, whatever its scores
-            const double all = row_any<LPR>(have, lane) ? -row_sum<LPR>(d, lane) / Z : 0.0;
+            // a row without a chosen filter has no gradient, whatever its scores, nor has one without an open filter
+            const double sum = row_sum<LPR>(d, lane);
+            const double all = (row_any<LPR>(have, lane) && m > minus_inf()) ? -sum / Z * A.score_scale : 0.0;
 #pragma unroll
-            for (int i = 0; i < VPL; i++) ds[i] = ds[i] == 0.0 ? 0.0 : ds[i] * all;
+            for (int i = 0; i < VPL; i++) ds[i] *= all;
         }
-        // a filter that is named twice gets both shares, in the order of the entries, from the first that names it
-        bool first = have;
-        double sum = 0;
-        for (int j = 0; j < A.k; j++) {
-            const int fj = __shfl(f, lane0 + j, 64);
-            const double dj = __shfl(d, lane0 + j, 64);
-            if (fj == f) {
-                sum += dj;
-                first &= j >= l;
+        d *= A.score_scale;
+        // The lane that finds its own number where it left it speaks for its filter.  One that does not shares it: a filter
+        // that is named twice (wn_route does not) gets both shares, in the order of the entries, from the first of them.
+        if (have) mine[f] = l;
+        route_lds_order();
+        bool first = have && mine[have ? f : 0] == l;
+        double sum = d;
+        if (__any(have && !first)) {
+            first = have;
+            sum = 0;
+            for (int j = 0; j < A.k; j++) {
+                const int fj = __shfl(f, lane0 + j, 64);
+                const double dj = __shfl(d, lane0 + j, 64);
+                if (fj == f) {
+                    sum += dj;
+                    first &= j >= l;
+                }
             }
         }
         if (first) mine[f] = sum;
@@ -912,10 +948,10 @@ __global__ __launch_bounds__(ROUTE_T) void k_route_backward(RouteArgs A) {
         if (first) mine[f] = 0;
         if (live) {
             switch (A.dtype) {
-                case WN_F64: store_chunk<double, VPL>(ds, A, row, f0); break;
-                case WN_F32: store_chunk<float, VPL>(ds, A, row, f0); break;
-                case WN_F16: store_chunk<f16_bits, VPL>(ds, A, row, f0); break;
-                default: store_chunk<bf16_bits, VPL>(ds, A, row, f0);
+                case WN_F64: store_chunk<double, LPR, VPL>(ds, A, row, f0); break;
+                case WN_F32: store_chunk<float, LPR, VPL>(ds, A, row, f0); break;
+                case WN_F16: store_chunk<f16_bits, LPR, VPL>(ds, A, row, f0); break;
+                default: store_chunk<bf16_bits, LPR, VPL>(ds, A, row, f0);
             }
         }
     }
@@ -1013,7 +1049,8 @@ int wn_route(wn_context* ctx, const void* scores_dev, int dtype, int T, int F, l
         }
         const RouteClass K = route_class(F, routing->k, dtype, bias_dev, routing->groups_kept < routing->groups);
         const int rows = wn::ROUTE_T / K.lpr;
-        const long long grid = std::max(1LL, std::min<long long>(((long long)T + rows - 1) / rows, (long long)ctx->numCU * 4));
+        // as many workgroups as are on the chip at a time: what they set up (biases, the first instructions) serves more rows
+        const long long grid = std::max(1LL, std::min<long long>(((long long)T + rows - 1) / rows, (long long)ctx->numCU * (F > 128 ? 3 : 6)));
         A.doubts = bias_dev || A.kept < A.groups || dtype == WN_F64;
         A.count_here = counts_dev && grid == 1 && !A.doubts;
         const size_t values = (size_t)(F + A.groups + 1) * sizeof(double);
