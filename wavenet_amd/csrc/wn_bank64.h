@@ -8,10 +8,10 @@
 
 namespace wn {
 
-// Above 16 taps the high-pass taps are signed low-pass taps, as in k_train64 (wn_wave64.h): coefficient (r, c) is then off by
+// From 16 taps on the high-pass taps are signed low-pass taps, as in k_train64 (wn_wave64.h): coefficient (r, c) is then off by
 // s_r s_c, s = sg on the high-pass indices and 1 on index 0.
 template <int NP>
-constexpr bool BANK_B_FROM_A = (NP > 16);
+constexpr bool BANK_B_FROM_A = (NP >= 16);
 template <int NP>
 __device__ __forceinline__ double bank_taps64(const double* taps, int N, double (&a)[NP], double (&b)[NP]) {
     bank_taps<NP>(taps, N, a, b);
