@@ -161,7 +161,8 @@ unsigned grid_for(wn_context* ctx, int B) { return (unsigned)std::min<long long>
 int launch_bank(wn_context* ctx, int NP, int sc, int kind, wn::BankArgs& A) {
     const size_t n = (size_t)1 << (A.lgR + A.lgC);
     if (ctx->wave64 && A.lgR == 6 && A.lgC == 6) {
-        // a workgroup per example, a wave per filter, up to the four waves whose tiles fit a CU
+        // a workgroup per example, a wave per filter, up to the four whose tiles fit a CU (2048 examples, 2 and 4 filters:
+        // forward 54 and 86 us; one wave for all of them in turn 66 and 114)
         const int waves = std::min(A.k, 4);
         // as many workgroups as are on the chip at a time, each fetching its next example early
         const unsigned grid = (unsigned)std::min(A.B, ctx->numCU * (4 / waves));
