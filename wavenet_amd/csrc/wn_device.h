@@ -134,6 +134,19 @@ __device__ __forceinline__ double block_sum(double v, double* red, int tid) {
     }
 }
 
+// Everything that the team's T threads wrote to LDS is there for all of them.  A team of one wave, alone in its workgroup or
+// beside others, waits for nobody: a wave's accesses to LDS are carried out in order, and only the compiler has to keep them so.
+template <int T>
+__device__ __forceinline__ void team_sync() {
+    if constexpr (T == 64) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    } else {
+        __syncthreads();
+    }
+}
+
 // ---------------------------------------------------------------------------------------------
 // One level of the forward cascade for NL = 2^lgNL lines (src/Wavenet.cxx:423-434):
 //   lo[k] = sum_j a[j] in[(N/2 + 2k - j) mod len],  hi[k] likewise with b.
@@ -193,16 +206,16 @@ __device__ __forceinline__ void fwd_pass(const double* in, double* P, double* ou
                                          const double (&a)[NP], const double (&b)[NP], int tid) {
     if (lgLen == 0) {  // a line of one sample is its own coefficient
         for (int w = tid; w < (1 << lgNL); w += T) { out[w * ls] = in[w * ls]; P[w * ls] = 0; }
-        __syncthreads();
+        team_sync<T>();
         return;
     }
     for (int i = lgLen - 1; i >= 0; i--) {
         const double* src = (i == lgLen - 1) ? in : P + (2 << i) * es;
         fwd_level<NP, T>(src, es, ls, P + (1 << i) * es, out + (1 << i) * es, lgNL, i, lanesOnLines, a, b, tid);
-        __syncthreads();
+        team_sync<T>();
     }
     for (int w = tid; w < (1 << lgNL); w += T) { out[w * ls] = P[w * ls + es]; P[w * ls] = 0; }
-    __syncthreads();
+    team_sync<T>();
 }
 
 template <int NP, int T>
@@ -212,7 +225,7 @@ __device__ __forceinline__ void fwd_pass_lo(const double* in, double* P, int es,
     for (int i = lgLen - 1; i >= 1; i--) {
         const double* src = (i == lgLen - 1) ? in : P + (2 << i) * es;
         fwd_level_lo<NP, T>(src, es, ls, P + (1 << i) * es, lgNL, i, lanesOnLines, a, tid);
-        __syncthreads();
+        team_sync<T>();
     }
 }
 
@@ -283,7 +296,7 @@ __device__ __forceinline__ void bwd_level(double* D, int es, int ls, const doubl
             no[it] = so;
         }
     }
-    __syncthreads();
+    team_sync<T>();
 #pragma unroll
     for (int it = 0; it < NIT; it++) {
         const int w = tid + it * T;
@@ -295,7 +308,7 @@ __device__ __forceinline__ void bwd_level(double* D, int es, int ls, const doubl
             D[line * ls + (2 * p + 1) * es] = no[it];
         }
     }
-    __syncthreads();
+    team_sync<T>();
 }
 
 // Backward pass over NL lines of length 2^lgLen.  `in` is the line the forward pass
