@@ -151,7 +151,6 @@ __device__ __forceinline__ double ckpt_max(double a, double b) { return (a > b |
 
 // ---- routed transforms --------------------------------------------------------------------------------------
 
-constexpr int BANK_MAX_TOPK = WN_MAX_TOPK;
 
 struct BankArgs {
     int B, lgR, lgC, k, F, N;
