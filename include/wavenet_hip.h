@@ -327,7 +327,7 @@ int wn_forward_routed(wn_context* ctx, const double* X_dev, int B, int R, int C,
  *     dfilters_dev[F][N]   sum of the gradients of the entries that name f (may be NULL)
  *     dw_dev[B][k]         <Delta, forward(X)> under filter idx[e][j] (may be NULL)
  *     dX_dev[B][n]         errors on the input (may be NULL)
- * Entries that name no filter have zero grad and dw.
+ * Entries that name no filter have zero grad and dw.  No output may overlap an input.
  */
 int wn_backprop_routed(wn_context* ctx, const double* Delta_dev, const double* X_dev, const signed char* q_dev, const float* scale_dev,
                        int B, int R, int C, const double* filters_dev, int F, int N, const int* idx_dev, const double* w_dev, int k,

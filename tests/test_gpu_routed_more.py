@@ -41,6 +41,55 @@ def test_workgroup_kernels_agree_with_the_one_wave_kernels(oracle, monkeypatch, 
     c.close()
 
 
+@pytest.mark.parametrize("N", [2, 6, 8, 16, 32])
+@pytest.mark.parametrize("R,C", [(32, 32), (16, 16), (64, 16), (1, 512), (1, 1024), (2, 512), (512, 2), (2, 256), (128, 8), (512, 1), (1024, 1)])
+@pytest.mark.parametrize("B,k", [(5, 3), (5, 5), (1100, 2)])
+def test_one_wave_transforms_in_lds(ctx, oracle, monkeypatch, R, C, N, B, k):
+    """Examples of 256 ... 1024 samples whose lines are short, long or single, signals among them where the register kernels
+    are off; few and many examples.  Bounds as in the other file: sums of up to 1024 products, errors relative to the largest."""
+    import torch
+    from wavenet_amd import Context
+    c = ctx
+    if C == 1:
+        monkeypatch.setenv("WAVENET_HIP_WAVE64", "0")
+        c = Context(0, stream=torch.cuda.current_stream().cuda_stream)
+    rng = np.random.default_rng(R + 5 * C + N)
+    F_ = 6
+    B = min(B, 1100 if N == 8 else 40)
+    X, D = rng.standard_normal((B, R, C)), rng.standard_normal((B, R, C))
+    bank = bank_of(F_, N, 17)
+    idx, w = entries(rng, B, F_, k)
+    assert near(run_forward(c, X, bank, idx, w, keep=False)[0], ref.forward(oracle, X, bank, idx, w))
+    for g, r in zip(run_backward(c, D, bank, idx, w, F_, N, X=X), ref.backward(oracle, D, X, bank, idx, w)):
+        assert near(g, r, 1e-10)
+    if c is not ctx:
+        c.close()
+
+
+@pytest.mark.parametrize("R,C", [(64, 64), (8, 8)])
+def test_outputs_over_inputs_are_refused(ctx, R, C):
+    import torch
+    from wavenet_amd.capi import WavenetError
+    B, n, N = 3, R * C, 4
+    bank, X = dev(bank_of(1, N, 2)), full((2 * B * n,), 1.5, torch.float64)
+    Y, grad, q, sc = (full((B * n,), 9.0, torch.float64), full((B * N,), 9.0, torch.float64), full((8 * B * n,), 3, torch.int8),
+                      full((B * -(-n // 64),), 0.5, torch.float32))
+    for at in (0, 1, B * n - 1):
+        with pytest.raises(WavenetError, match="overlap"):
+            ctx.forward_routed(X, B, R, C, bank, None, None, X[at:])
+        with pytest.raises(WavenetError, match="overlap"):
+            ctx.backprop_routed(Y, B, R, C, bank, None, None, grad, X=X, dX=X[at:])
+        with pytest.raises(WavenetError, match="overlap"):
+            ctx.backprop_routed(X, B, R, C, bank, None, None, grad, X=Y, dX=X[at:])
+    with pytest.raises(WavenetError, match="overlap"):
+        ctx.backprop_routed(Y, B, R, C, bank, None, None, grad, q=q, scales=sc, dX=q.view(torch.float64))
+    torch.cuda.synchronize()
+    assert (X == 1.5).all() and (Y == 9.0).all() and (grad == 9.0).all() and (q == 3).all()
+    ctx.forward_routed(X, B, R, C, bank, None, None, X[B * n:])     # one behind the other
+    torch.cuda.synchronize()
+    assert (X[:B * n] == 1.5).all()
+
+
 @pytest.mark.parametrize("R,C", [(64, 64), (256, 1), (8, 16)])
 @pytest.mark.parametrize("k", [3, 5, 8, 16])
 def test_more_filters_than_waves(ctx, oracle, R, C, k):

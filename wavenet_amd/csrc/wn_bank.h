@@ -151,7 +151,6 @@ __device__ __forceinline__ double ckpt_max(double a, double b) { return (a > b |
 
 // ---- routed transforms --------------------------------------------------------------------------------------
 
-
 struct BankArgs {
     int B, lgR, lgC, k, F, N;
     const double* filters;   // [F][N] taps
