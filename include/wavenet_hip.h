@@ -271,7 +271,7 @@ typedef struct wn_routing {
     int score;          /* WN_SCORE_SOFTMAX or WN_SCORE_SIGMOID */
     int k;              /* filters per example, 1 ... min(F, WN_MAX_TOPK) */
     int groups;         /* equal groups of consecutive filters (1: no groups; at most WN_MAX_GROUPS) */
-    int groups_kept;    /* groups a row chooses from (equal to groups: all) */
+    int groups_kept;    /* groups a row chooses from (equal to groups, of any number: all, as without groups) */
     int renormalise;    /* 1: the weights of a row add up to scale */
     double scale;       /* of the weights */
     double score_scale; /* of the scores, 1e-100 ... 1e100 either way; negative where a low score is a good one (sparsity costs) */

@@ -243,3 +243,44 @@ def test_another_stream_and_the_callers_device(oracle):
     some = np.r_[0:8]
     assert near(got[some], ref.forward(oracle, X[some], bank, idx[some], w[some]))
     c.close()
+
+
+@pytest.mark.parametrize("T,F_,k", [(5, 1024, 16), (700, 96, 3)])
+@pytest.mark.parametrize("dtype", ["float64", "float32", "bfloat16"])
+def test_all_groups_kept_is_no_groups(ctx, T, F_, k, dtype):
+    """Any number of groups, one per filter too, if all of them are kept."""
+    import torch
+    rng = np.random.default_rng(F_)
+    s = dev(rng.standard_normal((T, F_))).to(getattr(torch, dtype))
+    bias = dev(rng.standard_normal(F_) * 0.1)
+    for b in (None, bias):
+        want = run_route(ctx, s, k, bias=b)
+        for groups in (2, F_ // 3 if F_ % 3 == 0 else F_ // 4, F_):
+            got = run_route(ctx, s, k, bias=b, groups=groups, groups_kept=groups)
+            assert all(np.array_equal(g, w) for g, w in zip(got, want))
+
+
+def test_contexts_of_different_sizes(ctx):
+    """Two contexts on one GPU whose launches of the same kernels need different amounts of LDS, in turn."""
+    import torch
+    from wavenet_amd import Context
+    other = Context(0, stream=torch.cuda.current_stream().cuda_stream)
+    rng = np.random.default_rng(8)
+    big, small = dev(rng.standard_normal((40, 1024))), dev(rng.standard_normal((40, 640)))
+    bank = dev(bank_of(2, 4, 3))
+    X = [dev(rng.standard_normal((4, 64 * 64))) for _ in range(2)]
+    D = dev(rng.standard_normal((4, 64 * 64)))
+    first = None
+    for turn in range(3):
+        out = [run_route(c, s, 5, groups=16, groups_kept=4) for c, s in ((ctx, big), (other, small))]
+        for c, k in ((ctx, 4), (other, 2)):
+            idx = full((4, k), 1, torch.int32)
+            Y, grad, dX = full((4, 4096), 0.0, torch.float64), full((4, k, 4), 0.0, torch.float64), full((4, 4096), 0.0, torch.float64)
+            c.forward_routed(X[0], 4, 64, 64, bank, idx, None, Y)
+            c.backprop_routed(D, 4, 64, 64, bank, idx, None, grad, X=X[0], dX=dX)
+            torch.cuda.synchronize()
+            out.append([t.cpu().numpy() for t in (Y, grad, dX)])
+        if first is None:
+            first = out
+        assert all(np.array_equal(a, b) for x, y in zip(out, first) for a, b in zip(x, y))
+    other.close()

@@ -1021,7 +1021,8 @@ int check_routing(wn_context* ctx, const void* scores, int dtype, int T, int F, 
     if (!wn::aligned_to(scores, es)) return fail(ctx, WN_ERR_ARG, "misaligned pointer");
     A.scores = scores; A.dtype = dtype; A.rs = rs; A.cs = cs;
     A.T = T; A.F = F; A.k = r->k;
-    A.groups = r->groups; A.kept = r->groups_kept; A.per = F / r->groups;
+    const bool grouped = r->groups_kept < r->groups;         // all groups kept: none, whatever their number
+    A.groups = grouped ? r->groups : 1; A.kept = grouped ? r->groups_kept : 1; A.per = F / A.groups;
     A.per_magic = ((1u << 20) + A.per - 1) / A.per;
     A.sigmoid = r->score == WN_SCORE_SIGMOID; A.renorm = r->renormalise != 0;
     A.scale = r->scale; A.score_scale = r->score_scale;
