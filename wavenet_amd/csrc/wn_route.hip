@@ -192,17 +192,6 @@ __device__ __forceinline__ unsigned key_lane(unsigned v, int lane) {
     else return __shfl_xor(v, M, 64);
 }
 
-// the lowest of a whole number per lane
-template <int LPR>
-__device__ __forceinline__ int row_lowest(int v, int lane) {
-    v = min(v, (int)key_lane<1>((unsigned)v, lane));
-    v = min(v, (int)key_lane<2>((unsigned)v, lane));
-    v = min(v, (int)key_lane<7>((unsigned)v, lane));
-    v = min(v, (int)key_lane<8>((unsigned)v, lane));
-    if constexpr (LPR > 16) v = min(v, (int)key_lane<16>((unsigned)v, lane));
-    if constexpr (LPR > 32) v = min(v, (int)key_lane<32>((unsigned)v, lane));
-    return v;
-}
 // a whole number per lane added up over the row
 template <int LPR>
 __device__ __forceinline__ int row_count(int v, int lane) {
@@ -317,10 +306,16 @@ __device__ __forceinline__ unsigned long long kept_groups(T slack, const RouteAr
     double* grow = crow + A.F;
     for (int g = l; g < A.groups; g += LPR) {
         double first = minus_inf(), second = minus_inf();
-        for (int i = 0; i < A.per; i++) {
-            const double v = crow[g * A.per + i];
-            second = middle_of(first, second, v);
-            first = larger_of(first, v);
+        for (int i0 = 0; i0 < A.per; i0 += 4) {              // four on their way at a time
+            double v[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[i] = crow[g * A.per + min(i0 + i, A.per - 1)];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                v[i] = i0 + i < A.per ? v[i] : minus_inf();
+                second = middle_of(first, second, v[i]);
+                first = larger_of(first, v[i]);
+            }
         }
         grow[g] = second > minus_inf() ? first + second : first;
     }
@@ -328,11 +323,18 @@ __device__ __forceinline__ unsigned long long kept_groups(T slack, const RouteAr
     for (int g = l; g < A.groups; g += LPR) {
         const double mine = grow[g];
         int ahead = 0, surely = 0, perhaps = 0;
-        for (int h = 0; h < A.groups; h++) {
-            const double other = grow[h];
-            ahead += other > mine || (other == mine && h < g);
-            surely += other > mine + 2 * slack;
-            perhaps += other >= mine - 2 * slack && h != g;
+        for (int h0 = 0; h0 < A.groups; h0 += 4) {
+            double other[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) other[i] = grow[min(h0 + i, A.groups - 1)];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int h = h0 + i;
+                const bool there = h < A.groups;
+                ahead += there && (other[i] > mine || (other[i] == mine && h < g));
+                surely += there && other[i] > mine + 2 * slack;
+                perhaps += there && other[i] >= mine - 2 * slack && h != g;
+            }
         }
         doubt |= slack > 0 && mine > minus_inf() && surely < A.kept && perhaps >= A.kept;
         if (ahead < A.kept) keep |= 1ull << g;
@@ -598,8 +600,8 @@ __device__ __forceinline__ unsigned bits16(bf16_bits v) { return v.v; }
 __device__ __forceinline__ unsigned bits16(float) { return 0; }
 __device__ __forceinline__ unsigned bits16(double) { return 0; }
 
-// Three waves per SIMD and as many workgroups as that makes: 65536 x 256 bf16 scores with bias and groups 72 us; two waves
-// 75, one 94, four (with spills) 113.
+// Three waves per SIMD and as many workgroups as that makes: 65536 x 256 bf16 scores with bias and groups 52 us; two waves 55,
+// one 74, four (with spills) 93.
 template <class S, int LPR, int VPL, int K>
 __global__ __launch_bounds__(ROUTE_T, 3) void k_route32(RouteArgs A) {
     extern __shared__ __attribute__((aligned(16))) double route_lds[];
@@ -722,8 +724,9 @@ __global__ __launch_bounds__(ROUTE_T, 3) void k_route32(RouteArgs A) {
     count_here(A);
 }
 
-// A marked row in 64 bits and round by round, by one wave with the values in LDS: lane j < k returns its j-th filter.  Short
-// code before quick code: rows come here one at a time, and much of what that takes is the fetching of the instructions.
+// A marked row in 64 bits and round by round, by one wave with the values in LDS: lane j < k returns its j-th filter.  Rows
+// come here one at a time, so that a row's latency counts: for 256 scores with bias and groups some 2.8 k cycles for the
+// scores, 3.8 k for the shares, 4.9 k for the groups and 0.9 k a round (two exchanges, a write and a read of LDS each).
 __device__ __forceinline__ int choose_exactly(const RouteArgs& A, long long row, double* crow, int lane) {
     const bool shares = A.bias || A.kept < A.groups;
                 double m = minus_inf(), Z = 0;
@@ -761,25 +764,37 @@ __device__ __forceinline__ int choose_exactly(const RouteArgs& A, long long row,
                     }
                     route_lds_order();
                 }
-                int mine = -1;
+                // a lane keeps the best of its consecutive filters; only the one that gave it away looks again
+                const int own = (A.F + 63) / 64;
+                const auto look = [&](double& best, int& at) {
+                    best = minus_inf();
+                    for (int i0 = 0; i0 < own; i0 += 4) {    // four on their way at a time
+                        double v[4];
+#pragma unroll
+                        for (int i = 0; i < 4; i++) v[i] = crow[min(lane * own + i0 + i, A.F - 1)];
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const int f = lane * own + i0 + i;
+                            const bool better = i0 + i < own && f < A.F && v[i] > best;
+                            at = better ? f : at;
+                            best = better ? v[i] : best;
+                        }
+                    }
+                };
+                double best;
+                int at = 0, mine = -1;
+                look(best, at);
 #pragma nounroll
                 for (int j = 0; j < A.k; j++) {
-                    double best = minus_inf();
-                    int at = WN_MAX_EXPERTS;
-#pragma nounroll
-                    for (int f = lane; f < A.F; f += 64) {
-                        const double v = crow[f];
-                        at = v > best ? f : at;
-                        best = key_max(best, v);
-                    }
                     const double top = row_max<64>(best, lane);
-                    at = best == top && top > minus_inf() ? at : WN_MAX_EXPERTS;
-                    at = row_lowest<64>(at, lane);
-                    if (at < WN_MAX_EXPERTS) {
-                        if (lane == j) mine = at;
-                        if (lane == at % 64) crow[at] = minus_inf();
+                    if (!(top > minus_inf())) break;
+                    const int first = __builtin_ctzll(__ballot(best == top));    // the lowest lane has the lowest filter
+                    const int f = __builtin_amdgcn_readlane(at, first);
+                    if (lane == j) mine = f;
+                    if (lane == first) {
+                        crow[f] = minus_inf();
+                        look(best, at);
                     }
-                    route_lds_order();
                 }
     return mine;
 }
@@ -787,7 +802,10 @@ __device__ __forceinline__ int choose_exactly(const RouteArgs& A, long long row,
 // After k_route32 and k_route64: the rows that they marked (a workgroup's waves share its marked rows; equal values among
 // 16-bit scores under equal biases come here too, and may be many), and counts[f] += entries of idx that name f, by a
 // histogram per workgroup in LDS and one addition per filter (whole numbers, so that their order does not matter).
-constexpr int SETTLE_T = 1024;
+// 512 threads: with 1024 the registers spill, and setting up scratch memory alone takes every workgroup 8 k cycles (65536 x 256
+// bf16 with bias and groups 71 us against 64; 65536 x 64 with bias and groups 43 against 35); 256 have too few waves for many
+// marked rows (65536 x 1024 f32 with a bias: 197 us with 1024 threads, 208 with 512, 245 with 256).
+constexpr int SETTLE_T = 512;
 __global__ __launch_bounds__(SETTLE_T) void k_route_settle(RouteArgs A) {
     extern __shared__ __attribute__((aligned(16))) double route_lds[];
     __shared__ int hist[WN_MAX_EXPERTS], marked[SETTLE_T], marks;
