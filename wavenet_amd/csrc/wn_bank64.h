@@ -104,13 +104,14 @@ __device__ __forceinline__ double bank_max64(const double (&v)[64], int lane) {
     return m[0];
 }
 
-// Columns 4 m ... 4 m + 3 for the groups m = first, first + step, ... (the registers are indexed at compile time)
+// Columns 4 m ... 4 m + 3 for the groups m = first, first + step, ... (the registers are indexed at compile time), their scales
+// included: a maximum that lost a NaN is odd to the wave that quantises the NaN's column, and to no other.
 template <bool EXACT>
 __device__ __forceinline__ bool bank_keep64(const double (&v)[64], signed char* q, float* qs, int first, int step, int lane) {
     const float scale = ckpt_scale(bank_max64<EXACT>(v, lane));
     const double inv = ckpt_inverse(scale);
     bool odd = false;
-    if (first == 0) qs[lane] = scale;
+    if ((lane >> 2) % step == first) qs[lane] = scale;
     int* out = reinterpret_cast<int*>(q) + 16 * (lane & 3) + (lane >> 2);
     const int shift = 8 * (lane & 3);
     int turn = first;
