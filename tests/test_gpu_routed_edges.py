@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 import routed_ref as ref
-from test_gpu_routed import bank_of, run_backward, run_forward
+from test_gpu_routed import bank_of, dev, run_backward, run_forward, run_route
 
 pytestmark = pytest.mark.gpu
 
@@ -48,3 +48,24 @@ def test_kept_values_that_are_not_finite_under_several_filters(ctx, R, C, k, val
     grad, _, dw, _ = run_backward(ctx, D, bank, idx, w, 5, N, q=q, sc=sc)
     assert np.isnan(dw[:-1]).all() and np.isnan(grad[:-1]).any(axis=2).all()
     assert np.isfinite(dw[-1]).all() and np.isfinite(grad[-1]).all()
+
+
+# ---- router: values next to each other ------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("score_scale", [1.0, -1.0, 0.5])
+@pytest.mark.parametrize("F_,k", [(2, 1), (8, 1), (8, 3), (60, 16), (256, 8), (1000, 16)])
+def test_route_orders_the_smallest_scores(ctx, F_, k, score_scale):
+    """Scores a few units of the smallest 64-bit number apart, of either sign, among zeros, and where normal numbers begin."""
+    rng = np.random.default_rng(F_ + k)
+    unit = 5e-324
+    rows = [rng.integers(-m, m + 1, (12, F_)) * unit for m in (1, 3, 40, 1023, 2050, 5000)]
+    rows.append((2 ** 52 + rng.integers(-1500, 1500, (12, F_))) * unit)
+    rows.append(-(2 ** 53 + rng.integers(0, 1500, (12, F_))) * unit)
+    zeros = np.zeros((4, F_))
+    zeros[0, -1], zeros[1, -1], zeros[2, 0], zeros[3, F_ // 2] = 1e-321, unit, -unit, 1022 * unit
+    s = np.concatenate(rows + [zeros])
+    for kw in (dict(), dict(score="sigmoid"), dict(groups=2, groups_kept=1, renormalise=False)):
+        idx, w, counts = run_route(ctx, dev(s), k, score_scale=score_scale, **kw)
+        ri, rw, rc = ref.route(s, k, score_scale=score_scale, **kw)
+        assert np.array_equal(idx, ri) and np.array_equal(counts, rc)
+        assert np.allclose(w, rw, rtol=2000 * 2.0 ** -53, atol=0)

@@ -529,12 +529,14 @@ __global__ __launch_bounds__(ROUTE_T) void k_route64(RouteArgs A) {
         const int f = mine > minus_inf() ? filter_of(mine) : -1;
         if (!as_read) {
             // Values this close may have changed places.  Of the chosen ones neighbours are looked at, around the last of
-            // them every value; equal ones stand in order of the filter already.
+            // them every value; equal ones stand in order of the filter already.  The bits given up are 2^-42 of a value, or
+            // less than 1024 of the smallest numbers where values are no larger than 2^-1022.
+            constexpr double SMALLEST = 2048 * 0x1p-1074;
             const double own = f >= 0 ? A.score_scale * score_at(A, row, f) : 0.0;
             const double next_own = __shfl_down(own, 1, 64), next = __shfl_down(mine, 1, 64);
             doubt |= l + 1 < A.k && next > minus_inf() && own != next_own &&
-                     mine - next <= 0x1p-40 * __builtin_fmax(__builtin_fabs(mine), __builtin_fabs(next));
-            const double at_last = __shfl(own, (lane - l) + A.k - 1, 64), slack = 0x1p-40 * __builtin_fabs(last);
+                     mine - next <= 0x1p-40 * __builtin_fmax(__builtin_fabs(mine), __builtin_fabs(next)) + SMALLEST;
+            const double at_last = __shfl(own, (lane - l) + A.k - 1, 64), slack = 0x1p-40 * __builtin_fabs(last) + SMALLEST;
 #pragma unroll
             for (int i = 0; i < VPL; i++) doubt |= last > minus_inf() && c[i] != at_last && c[i] >= last - slack && c[i] <= last + slack;
         }
