@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 import routed_ref as ref
-from test_gpu_routed import bank_of, dev, run_backward, run_forward, run_route
+from test_gpu_routed import bank_of, dev, host, run_backward, run_forward, run_route
 
 pytestmark = pytest.mark.gpu
 
@@ -69,3 +69,36 @@ def test_route_orders_the_smallest_scores(ctx, F_, k, score_scale):
         ri, rw, rc = ref.route(s, k, score_scale=score_scale, **kw)
         assert np.array_equal(idx, ri) and np.array_equal(counts, rc)
         assert np.allclose(w, rw, rtol=2000 * 2.0 ** -53, atol=0)
+
+
+def test_route_chosen_again_in_groups_and_counted(ctx):
+    """Rows that the 32-bit values leave in doubt, most of a batch: the counts are those of the indices that left, and a row that
+    differs from the reference holds values that 64 bits do not tell apart.  p is within 2000 * 2^-53 of itself (as the weights
+    are), p + bias rounds by half a unit of 2^-52 |c| on either side, a group's score is the sum of two."""
+    import torch
+    rng = np.random.default_rng(9)
+    for T, F_, k, groups in ((600, 256, 8, 16), (777, 40, 5, 8), (100, 600, 16, 30)):
+        wide = rng.standard_normal((T, F_))
+        for scores, dtype in ((wide * 1.5, torch.bfloat16), (wide * 40.0, torch.bfloat16), (wide * 40.0, torch.float32), (wide * 40.0, torch.float64)):
+            s = dev(scores).to(dtype)
+            for bias in (None, np.zeros(F_), rng.integers(0, 2, F_) * 1e-7, rng.standard_normal(F_) * 1e6):
+                for kw in (dict(score="sigmoid", groups=groups, groups_kept=3), dict(groups=groups, groups_kept=2)):
+                    idx, w, counts = run_route(ctx, s, k, bias=None if bias is None else dev(bias), **kw)
+                    assert np.array_equal(counts, np.bincount(idx[idx >= 0], minlength=F_))
+                    ri, rw, _ = ref.route(host(s), k, bias=bias, **kw)
+                    same = (idx == ri).all(axis=1)
+                    assert np.allclose(w[same], rw[same], rtol=2000 * 2.0 ** -53, atol=0)
+                    if same.all():
+                        continue
+                    p = ref.shares(host(s), kw.get("score", "softmax"))
+                    c = p if bias is None else p + bias
+                    bound = 2 * (2 * 2000 * 2.0 ** -53 + 4 * 2.0 ** -53 * np.abs(c).max())
+                    best = np.sort(c.reshape(T, groups, -1), axis=2)[:, :, -2:].sum(axis=2)
+                    order = np.sort(best, axis=1)[:, ::-1]
+                    kept = kw["groups_kept"]
+                    for t in np.flatnonzero(~same):
+                        assert (idx[t] >= 0).all() and len(set(idx[t])) == k
+                        near_groups = order[t, kept - 1] - order[t, kept] <= bound
+                        # (without a bias filters of a group are told apart by their scores, which are exact)
+                        near_values = bias is not None and (np.abs(c[t, idx[t]] - c[t, ri[t]]) <= bound).all()
+                        assert near_groups or near_values, (T, kw, t)
