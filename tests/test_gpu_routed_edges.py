@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 import routed_ref as ref
-from test_gpu_routed import bank_of, dev, host, run_backward, run_forward, run_route
+from test_gpu_routed import bank_of, dev, full, host, run_backward, run_forward, run_route
 
 pytestmark = pytest.mark.gpu
 
@@ -102,3 +102,19 @@ def test_route_chosen_again_in_groups_and_counted(ctx):
                         # (without a bias filters of a group are told apart by their scores, which are exact)
                         near_values = bias is not None and (np.abs(c[t, idx[t]] - c[t, ri[t]]) <= bound).all()
                         assert near_groups or near_values, (T, kw, t)
+
+
+# ---- refusals -------------------------------------------------------------------------------------------------------
+
+def test_a_refused_backward_pass_has_written_nothing(ctx):
+    import torch
+    from wavenet_amd import capi
+    B, n, N = 3, 64, 4
+    D, X, bank = full((B, n), 1.0, torch.float64), full((B, n), 2.0, torch.float64), dev(bank_of(2, N, 0))
+    grad, dw, dX = full((B, 1, N), 9.0, torch.float64), full((B, 1), 9.0, torch.float64), full((B, n), 9.0, torch.float64)
+    dF = full((2 * N + 1,), 9.0, torch.float64)
+    with pytest.raises(capi.WavenetError) as err:
+        ctx.backprop_routed(D, B, 8, 8, bank, None, None, grad, X=X, dw=dw, dX=dX, dfilters=dF.data_ptr() + 4)
+    assert err.value.status == capi.WN_ERR_ARG
+    torch.cuda.synchronize()
+    assert all((t == 9.0).all() for t in (grad, dw, dX, dF))

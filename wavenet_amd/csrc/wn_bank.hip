@@ -216,6 +216,7 @@ int wn_backprop_routed(wn_context* ctx, const double* Delta_dev, const double* X
         int NP, sc;
         int rc = check_bank(ctx, B, R, C, filters_dev, F, N, idx_dev, w_dev, k, A, NP, sc);
         if (rc) return rc;
+        if (!wn::aligned_to(dfilters_dev, 8)) return fail(ctx, WN_ERR_ARG, "misaligned pointer");
         if (B > 0) {
             if (!Delta_dev || !grad_dev) return fail(ctx, WN_ERR_ARG, "null pointer");
             if (!q_dev != !scale_dev) return fail(ctx, WN_ERR_ARG, "a checkpoint is values and scales");
@@ -231,7 +232,6 @@ int wn_backprop_routed(wn_context* ctx, const double* Delta_dev, const double* X
             if (rc) return rc;
         }
         if (!dfilters_dev) return WN_OK;
-        if (!wn::aligned_to(dfilters_dev, 8)) return fail(ctx, WN_ERR_ARG, "misaligned pointer");
         wn::BankReduceArgs S = {idx_dev, grad_dev, dfilters_dev, (long long)B * k, N};
         return wn::launch_kernel(ctx, reduce_for(NP), (unsigned)F, wn::reduce_threads(NP), 0, S);
     });
