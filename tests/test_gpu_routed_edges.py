@@ -118,3 +118,29 @@ def test_a_refused_backward_pass_has_written_nothing(ctx):
     assert err.value.status == capi.WN_ERR_ARG
     torch.cuda.synchronize()
     assert all((t == 9.0).all() for t in (grad, dw, dX, dF))
+
+
+def test_layouts_other_than_the_strides_are_refused(ctx):
+    """A tensor whose own strides are not the ones passed would be read as other values than the caller's."""
+    import torch
+    rng = np.random.default_rng(0)
+    T, F_, k = 12, 8, 2
+    s = rng.standard_normal((T, F_))
+    idx, w = full((T, k), 0, torch.int32), full((T, k), 0.0, torch.float64)
+    turned, gaps = dev(s.T.copy()).t(), dev(np.repeat(s, 2, axis=1))[:, ::2]
+    ri, rw, _ = ref.route(s, k)
+    for v in (turned, gaps):
+        with pytest.raises(ValueError, match="strides"):
+            ctx.route(v, T, F_, idx, w, k=k)
+        with pytest.raises(ValueError, match="strides"):
+            ctx.route_backward(dev(s), T, F_, idx, w, v, k=k)
+        with pytest.raises(ValueError, match="strides"):
+            ctx.route_backward(v, T, F_, idx, w, dev(s), k=k)
+        with pytest.raises(ValueError, match="strides"):
+            ctx.checkpoint_pack(v, T, F_, full((T, F_), 0, torch.int8), full((T, 1), 0.0, torch.float32))
+        with pytest.raises(ValueError, match="strides"):
+            ctx.checkpoint_unpack(full((T, F_), 0, torch.int8), full((T, 1), 0.0, torch.float32), T, F_, v)
+        gi, gw, _ = run_route(ctx, v, k)                            # with its strides
+        assert np.array_equal(gi, ri) and np.allclose(gw, rw, rtol=2000 * 2.0 ** -53, atol=0)
+    with pytest.raises(ValueError, match="strides"):
+        ctx.route(turned, T, F_, idx, w, k=k, row_stride=1, col_stride=F_)      # (a column is T scores long)

@@ -172,6 +172,20 @@ def _dtype_code(x, dtype):
     return _TYPE_CODES.get(dtype, dtype)
 
 
+def _strided(x, rows, row_stride, cols, col_stride):
+    """Whether a tensor that is not contiguous holds value (r, c) where the strides say: both have to be strides of its
+    dimensions, or of neighbouring dimensions that make one."""
+    if x.dim() == 2 and x.stride() == (row_stride, col_stride):
+        return x.shape[0] >= rows and x.shape[1] >= cols
+    dims = [(n, s) for n, s in zip(x.shape, x.stride()) if n > 1]
+    runs, n, s = [], 0, 0
+    for m, t in reversed(dims):
+        n, s = (n * m, s) if n and t == n * s else (m, t)
+        runs.append((n, s))
+    return all(count <= 1 or any(s == stride and n >= count for n, s in dims + runs)
+               for count, stride in ((rows, row_stride), (cols, col_stride)))
+
+
 # --- host-only entry points ----------------------------------------------------------------------
 
 def reg_term(a, wavelet=True):
@@ -291,21 +305,28 @@ class Context:
                                                  f.shape[1], _addr(S)))
 
     # routed filter bank ---------------------------------------------------------------------------
-    def _buffer(self, name, x, count, wanted=None, span=None):
-        """Address of an argument.  A tensor has to lie on the context's GPU, hold `count` elements (or with `span` reach
-        that far from its first) of the type, densely; an address is taken as it is."""
+    def _buffer(self, name, x, count, wanted=None, strides=None):
+        """Address of an argument.  A tensor has to lie on the context's GPU and hold `count` elements of the type, densely,
+        or with `strides` (rows, row_stride, cols, col_stride) reach the last of them, with these strides unless it is
+        contiguous; an address is taken as it is."""
         if x is None or isinstance(x, int):
             return x
         if not x.is_cuda or x.get_device() != self.device:
             raise ValueError(f"{name} is on {x.device}, the context on GPU {self.device}")
         if wanted is not None and _type_name(x) != wanted:
             raise ValueError(f"{name} holds {_type_name(x)}, not {wanted}")
-        if span is None:
+        if strides is None:
             if not x.is_contiguous():
                 raise ValueError(f"{name} is not contiguous")
             if x.numel() < count:
                 raise ValueError(f"{name} holds {x.numel()} elements, {count} are needed")
-        elif not x.is_contiguous() or x.numel() < span:
+            return x.data_ptr()
+        rows, row_stride, cols, col_stride = strides
+        span = (rows - 1) * row_stride + (cols - 1) * col_stride + 1 if rows > 0 and cols > 0 else 0
+        dense = x.is_contiguous()
+        if not dense or x.numel() < span:
+            if not dense and span > 0 and not _strided(x, *strides):
+                raise ValueError(f"{name} has strides {tuple(x.stride())}, not {row_stride} between rows and {col_stride} in them")
             held = x.untyped_storage().nbytes() // x.element_size() - x.storage_offset()
             if held < span:
                 raise ValueError(f"{name} ends {held} elements after its start, {span} are needed")
@@ -328,10 +349,10 @@ class Context:
         score (t, f) lies t * row_stride + f * col_stride elements from the start (default: dense rows).
         idx: int32 [T][k], w: float64 [T][k], bias: float64 [F], counts: int32 [F]."""
         rs = F * col_stride if row_stride is None else row_stride
-        span = (T - 1) * rs + (F - 1) * col_stride + 1 if T > 0 else 0
+        at = (T, rs, F, col_stride)
         r = self._routing(k, score, groups, groups_kept, renormalise, scale, score_scale)
         self._check(self.lib.wn_route(
-            self._h, self._buffer("scores", scores, 0, span=span), _dtype_code(scores, dtype), T, F, rs, col_stride, C.byref(r),
+            self._h, self._buffer("scores", scores, 0, strides=at), _dtype_code(scores, dtype), T, F, rs, col_stride, C.byref(r),
             self._buffer("bias", bias, F, "float64"), self._buffer("idx", idx, T * k, "int32"),
             self._buffer("w", w, T * k, "float64"), self._buffer("counts", counts, F, "int32")))
 
@@ -339,21 +360,21 @@ class Context:
                        scale=1.0, score_scale=1.0, row_stride=None, col_stride=1, dtype=None):
         """wn_route_backward: gradient dw of the weights -> gradient of the scores, laid out as the scores."""
         rs = F * col_stride if row_stride is None else row_stride
-        span = (T - 1) * rs + (F - 1) * col_stride + 1 if T > 0 else 0
+        at = (T, rs, F, col_stride)
         r = self._routing(k, score, groups, groups_kept, renormalise, scale, score_scale)
         code = _dtype_code(scores, dtype)
         if _dtype_code(dscores, dtype if isinstance(dscores, int) else None) != code and dscores is not None and not isinstance(dscores, int):
             raise ValueError("dscores and scores differ in type")
         self._check(self.lib.wn_route_backward(
-            self._h, self._buffer("scores", scores, 0, span=span), code, T, F, rs, col_stride, C.byref(r),
+            self._h, self._buffer("scores", scores, 0, strides=at), code, T, F, rs, col_stride, C.byref(r),
             self._buffer("idx", idx, T * k, "int32"), self._buffer("dw", dw, T * k, "float64"),
-            self._buffer("dscores", dscores, 0, span=span)))
+            self._buffer("dscores", dscores, 0, strides=at)))
 
     def checkpoint_pack(self, X, B, n, q, scales, row_stride=None, dtype=None):
         """wn_checkpoint_pack: B rows of n values as int8 q[B][n] and float32 scales[B][ceil(n / 64)]."""
         rs = n if row_stride is None else row_stride
         self._check(self.lib.wn_checkpoint_pack(
-            self._h, self._buffer("X", X, 0, span=(B - 1) * rs + n if B > 0 else 0), _dtype_code(X, dtype), B, n, rs,
+            self._h, self._buffer("X", X, 0, strides=(B, rs, n, 1)), _dtype_code(X, dtype), B, n, rs,
             self._buffer("q", q, B * n, "int8"), self._buffer("scales", scales, B * -(-n // 64), "float32")))
 
     def checkpoint_unpack(self, q, scales, B, n, X, row_stride=None, dtype=None):
@@ -361,7 +382,7 @@ class Context:
         rs = n if row_stride is None else row_stride
         self._check(self.lib.wn_checkpoint_unpack(
             self._h, self._buffer("q", q, B * n, "int8"), self._buffer("scales", scales, B * -(-n // 64), "float32"),
-            _dtype_code(X, dtype), B, n, rs, self._buffer("X", X, 0, span=(B - 1) * rs + n if B > 0 else 0)))
+            _dtype_code(X, dtype), B, n, rs, self._buffer("X", X, 0, strides=(B, rs, n, 1))))
 
     def _bank(self, filters, F, N):
         """(filters, F, N): a tensor [F][N] says both numbers; None is the context's own filter."""
