@@ -144,3 +144,32 @@ def test_layouts_other_than_the_strides_are_refused(ctx):
         assert np.array_equal(gi, ri) and np.allclose(gw, rw, rtol=2000 * 2.0 ** -53, atol=0)
     with pytest.raises(ValueError, match="strides"):
         ctx.route(turned, T, F_, idx, w, k=k, row_stride=1, col_stride=F_)      # (a column is T scores long)
+
+
+def test_tables_of_another_width_are_refused(ctx):
+    """Indices, weights and filters of two dimensions are rows of k and of N: any other width would be read out of step."""
+    import torch
+    B, n, N = 6, 64, 4
+    X, Y, bank = full((B, n), 1.0, torch.float64), full((B, n), 9.0, torch.float64), dev(bank_of(3, N, 0))
+    two, three = full((B, 2), 0, torch.int32), full((B, 3), 0, torch.int32)
+    w2, w3 = full((B, 2), 9.0, torch.float64), full((B, 3), 9.0, torch.float64)
+    grad = full((B, 2, N), 9.0, torch.float64)
+    s = full((B, 8), 0.0, torch.float64)
+    with pytest.raises(ValueError, match="wide"):
+        ctx.forward_routed(X, B, 8, 8, bank, two, w3, Y)
+    with pytest.raises(ValueError, match="wide"):
+        ctx.forward_routed(X, B, 8, 8, bank, three, w3, Y, k=2)
+    with pytest.raises(ValueError, match="wide"):
+        ctx.forward_routed(X, B, 8, 8, bank, two, w2, Y, N=2)
+    for kw in (dict(dw=w3), dict(grad=full((B, 3, N), 9.0, torch.float64)), dict(grad=full((B, 2, N + 1), 9.0, torch.float64)),
+               dict(dfilters=full((3, N + 2), 9.0, torch.float64))):
+        with pytest.raises(ValueError, match="wide"):
+            ctx.backprop_routed(Y, B, 8, 8, bank, two, w2, **{"grad": grad, "X": X, **kw})
+    with pytest.raises(ValueError, match="wide"):
+        ctx.route(s, B, 8, three, w2, k=2)
+    with pytest.raises(ValueError, match="wide"):
+        ctx.route(s, B, 8, two, w3, k=2)
+    with pytest.raises(ValueError, match="wide"):
+        ctx.route_backward(s, B, 8, two, w3, s.clone(), k=2)
+    torch.cuda.synchronize()
+    assert (Y == 9.0).all() and (grad == 9.0).all() and (w2 == 9.0).all() and not two.any()

@@ -186,6 +186,18 @@ def _strided(x, rows, row_stride, cols, col_stride):
                for count, stride in ((rows, row_stride), (cols, col_stride)))
 
 
+def _out_of_step(x, count, *widths):
+    """Whether a tensor of rows, with more elements than the `count` of the table it is taken for, has rows of another width."""
+    if x is None or isinstance(x, int) or x.dim() < 2 or x.shape[0] < 2 or x.numel() == count:
+        return False
+    return x.numel() // x.shape[0] not in widths
+
+
+def _check_width(name, x, count, *widths):
+    if _out_of_step(x, count, *widths):
+        raise ValueError(f"{name} is {x.numel() // x.shape[0]} wide, not {widths[0]}")
+
+
 # --- host-only entry points ----------------------------------------------------------------------
 
 def reg_term(a, wavelet=True):
@@ -351,6 +363,8 @@ class Context:
         rs = F * col_stride if row_stride is None else row_stride
         at = (T, rs, F, col_stride)
         r = self._routing(k, score, groups, groups_kept, renormalise, scale, score_scale)
+        _check_width("idx", idx, T * k, k, 1)
+        _check_width("w", w, T * k, k, 1)
         self._check(self.lib.wn_route(
             self._h, self._buffer("scores", scores, 0, strides=at), _dtype_code(scores, dtype), T, F, rs, col_stride, C.byref(r),
             self._buffer("bias", bias, F, "float64"), self._buffer("idx", idx, T * k, "int32"),
@@ -365,6 +379,8 @@ class Context:
         code = _dtype_code(scores, dtype)
         if _dtype_code(dscores, dtype if isinstance(dscores, int) else None) != code and dscores is not None and not isinstance(dscores, int):
             raise ValueError("dscores and scores differ in type")
+        _check_width("idx", idx, T * k, k, 1)
+        _check_width("dw", dw, T * k, k, 1)
         self._check(self.lib.wn_route_backward(
             self._h, self._buffer("scores", scores, 0, strides=at), code, T, F, rs, col_stride, C.byref(r),
             self._buffer("idx", idx, T * k, "int32"), self._buffer("dw", dw, T * k, "float64"),
@@ -395,6 +411,7 @@ class Context:
             N = filters.shape[1] if N is None else N
         if F is None or N is None:
             raise ValueError("the number of filters and of taps is not known: pass a tensor [F][N], or F and N")
+        _check_width("filters", filters, F * N, N)
         return self._buffer("filters", filters, F * N, "float64"), F, N
 
     @staticmethod
@@ -411,6 +428,8 @@ class Context:
         (None: ones); q, scales: where to keep the checkpoint of X, if wanted."""
         filters, F, N = self._bank(filters, F, N)
         k, n = self._entries(idx, w, k), R * Cc
+        _check_width("idx", idx, B * k, k, 1)
+        _check_width("w", w, B * k, k, 1)
         self._check(self.lib.wn_forward_routed(
             self._h, self._buffer("X", X, B * n, "float64"), B, R, Cc, filters, F, N, self._buffer("idx", idx, B * k, "int32"),
             self._buffer("w", w, B * k, "float64"), k, self._buffer("Y", Y, B * n, "float64"), self._buffer("q", q, B * n, "int8"),
@@ -422,6 +441,10 @@ class Context:
         the checkpoint (q, scales) that forward_routed or checkpoint_pack kept."""
         filters, F, N = self._bank(filters, F, N)
         k, n = self._entries(idx, w, k), R * Cc
+        for name, x in (("idx", idx), ("w", w), ("dw", dw)):
+            _check_width(name, x, B * k, k, 1)
+        _check_width("grad", grad, B * k * N, k * N, N)
+        _check_width("dfilters", dfilters, F * N, N)
         self._check(self.lib.wn_backprop_routed(
             self._h, self._buffer("Delta", Delta, B * n, "float64"), self._buffer("X", X, B * n, "float64"),
             self._buffer("q", q, B * n, "int8"), self._buffer("scales", scales, B * -(-n // 64), "float32"), B, R, Cc, filters, F, N,
