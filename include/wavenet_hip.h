@@ -316,7 +316,7 @@ int wn_checkpoint_unpack(wn_context* ctx, const signed char* q_dev, const float*
  * the context's own filter).  idx_dev[B][k], w_dev[B][k] as wn_route leaves them; idx_dev NULL (k = 1) is filter 0
  * throughout, w_dev NULL is ones.  An entry outside 0 ... F - 1 names no filter and adds 0 * w.  The same filter may be
  * named twice.  q_dev and scale_dev (both or neither) receive the checkpoint of X, as wn_checkpoint_pack of B rows of
- * R * C values.  Examples of up to WN_MAX_FUSED samples.  Y_dev may not overlap the inputs.
+ * R * C values.  Examples of up to WN_MAX_FUSED samples.  No output may overlap an input or another output.
  */
 int wn_forward_routed(wn_context* ctx, const double* X_dev, int B, int R, int C, const double* filters_dev, int F, int N,
                       const int* idx_dev, const double* w_dev, int k, double* Y_dev, signed char* q_dev, float* scale_dev);
@@ -327,7 +327,7 @@ int wn_forward_routed(wn_context* ctx, const double* X_dev, int B, int R, int C,
  *     dfilters_dev[F][N]   sum of the gradients of the entries that name f (may be NULL)
  *     dw_dev[B][k]         <Delta, forward(X)> under filter idx[e][j] (may be NULL)
  *     dX_dev[B][n]         errors on the input (may be NULL)
- * Entries that name no filter have zero grad and dw.  No output may overlap an input.
+ * Entries that name no filter have zero grad and dw.  No output may overlap an input or another output.
  */
 int wn_backprop_routed(wn_context* ctx, const double* Delta_dev, const double* X_dev, const signed char* q_dev, const float* scale_dev,
                        int B, int R, int C, const double* filters_dev, int F, int N, const int* idx_dev, const double* w_dev, int k,

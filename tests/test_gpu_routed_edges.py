@@ -173,3 +173,51 @@ def test_tables_of_another_width_are_refused(ctx):
         ctx.route_backward(s, B, 8, two, w3, s.clone(), k=2)
     torch.cuda.synchronize()
     assert (Y == 9.0).all() and (grad == 9.0).all() and (w2 == 9.0).all() and not two.any()
+
+
+@pytest.mark.parametrize("from_checkpoint", [False, True])
+def test_every_output_over_every_other_argument_is_refused(ctx, from_checkpoint):
+    """By a byte at either end; what lies side by side is taken, and a refused call has written nothing."""
+    import torch
+    from wavenet_amd import capi
+    B, R, C, N, F_, k = 3, 8, 16, 4, 5, 2
+    n, nb = R * C, R * C // 64
+    nbytes = dict(X=8 * B * n, filters=8 * F_ * N, idx=4 * B * k, w=8 * B * k, Y=8 * B * n, q=B * n, scales=4 * B * nb, Delta=8 * B * n,
+                  grad=8 * B * k * N, dfilters=8 * F_ * N, dw=8 * B * k, dX=8 * B * n)
+    align = dict(idx=4, scales=4, q=1)
+    room = 64 * (sum(nbytes.values()) // 64 + 2 * len(nbytes))
+    # the arguments of one call after the other, without a gap but for alignment
+    arena = torch.zeros(3 * room, dtype=torch.uint8, device="cuda")
+    base, at, end = arena.data_ptr(), {}, arena.data_ptr() + room
+    for name, size in sorted(nbytes.items(), key=lambda item: -align.get(item[0], 8)):
+        at[name] = end
+        end += size
+    used = end - base
+
+    def forward(a):
+        ctx.forward_routed(a["X"], B, R, C, a["filters"], a["idx"], a["w"], a["Y"], k=k, F=F_, N=N, q=a["q"], scales=a["scales"])
+
+    def backward(a):
+        src = dict(q=a["q"], scales=a["scales"]) if from_checkpoint else dict(X=a["X"])
+        ctx.backprop_routed(a["Delta"], B, R, C, a["filters"], a["idx"], a["w"], a["grad"], dfilters=a["dfilters"], dw=a["dw"], dX=a["dX"], k=k,
+                            F=F_, N=N, **src)
+
+    back_in = ["Delta", "filters", "idx", "w"] + (["q", "scales"] if from_checkpoint else ["X"])
+    tried = 0
+    for call, outputs, inputs in ((forward, ["Y", "q", "scales"], ["X", "filters", "idx", "w"]), (backward, ["grad", "dfilters", "dw", "dX"], back_in)):
+        call(at)
+        torch.cuda.synchronize()
+        before = arena.clone()
+        for o in outputs:
+            for other in [x for x in inputs + outputs if x != o]:
+                step = align.get(o, 8)
+                first = at[other] - nbytes[o] + step                    # the last element of o on the first of the other
+                last = at[other] + nbytes[other] - step                 # and the other way round
+                for address in (first + -(first - base) % step, last - (last - base) % step, at[other] + -(at[other] - base) % step):
+                    with pytest.raises(capi.WavenetError, match="overlaps") as err:
+                        call({**at, o: address})
+                    assert err.value.status == capi.WN_ERR_ARG
+                    tried += 1
+        torch.cuda.synchronize()
+        assert torch.equal(arena, before)
+    assert tried >= 3 * 3 * 6 and used <= arena.numel()

@@ -5,6 +5,7 @@
 #include <hip/hip_runtime.h>
 
 #include <exception>
+#include <initializer_list>
 #include <string>
 
 #include "wavenet_hip.h"
@@ -66,6 +67,34 @@ int launch_kernel(wn_context* ctx, const void* func, unsigned grid, unsigned thr
 }
 
 inline bool aligned_to(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
+// Memory of an argument: `pieces` of `bytes` each, `stride` bytes apart (at least a piece); a null pointer is none.
+struct Memory {
+    const char* name;
+    const void* at;
+    unsigned long long bytes, pieces = 1, stride = 0;
+};
+// whether the first, in one piece, shares a byte with the second
+inline bool meets(const Memory& a, const Memory& b) {
+    if (!a.at || !b.at || !a.bytes || !b.bytes || !b.pieces) return false;
+    const unsigned long long x = (uintptr_t)a.at, y = (uintptr_t)b.at;
+    // the first piece that ends behind the start of a
+    const unsigned long long i = x < y + b.bytes ? 0 : b.pieces == 1 ? 1 : (x - y - b.bytes) / b.stride + 1;
+    return i < b.pieces && y + i * b.stride < x + a.bytes;
+}
+// No output may lie in an input or in another output.  Either is in one piece, or all that it is compared with are.
+inline int refuse_overlaps(wn_context* ctx, std::initializer_list<Memory> outputs, std::initializer_list<Memory> inputs) {
+    const auto refuse = [&](const Memory& o, const Memory& m) {
+        return fail(ctx, WN_ERR_ARG, std::string(o.name) + " overlaps " + m.name);
+    };
+    for (const Memory* o = outputs.begin(); o != outputs.end(); o++) {
+        for (const Memory& i : inputs)
+            if (o->pieces > 1 ? meets(i, *o) : meets(*o, i)) return refuse(*o, i);
+        for (const Memory* p = o + 1; p != outputs.end(); p++)
+            if (o->pieces > 1 ? meets(*p, *o) : meets(*o, *p)) return refuse(*o, *p);
+    }
+    return WN_OK;
+}
 
 inline size_t element_bytes(int dtype) {
     switch (dtype) {

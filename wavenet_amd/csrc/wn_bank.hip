@@ -158,11 +158,14 @@ int check_bank(wn_context* ctx, int B, int R, int C, const double* filters, int 
     return WN_OK;
 }
 
-// [a, a + bytes) and [b, b + b_bytes) share memory; null shares none
-bool overlap(const void* a, size_t bytes, const void* b, size_t b_bytes) {
-    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
-    return a && b && x < y + b_bytes && y < x + bytes;
-}
+// sizes of a call's arguments, in elements
+struct BankMemory {
+    unsigned long long values, entries, bank;   // of X and the like, of idx and w, of the filters
+    unsigned long long blocks;                  // of a checkpoint
+    BankMemory(const wn::BankArgs& A)
+        : values((unsigned long long)A.B << (A.lgR + A.lgC)), entries((unsigned long long)A.B * A.k), bank((unsigned long long)A.F * A.N),
+          blocks((unsigned long long)A.B * (((1ull << (A.lgR + A.lgC)) + wn::CKPT_BLOCK - 1) / wn::CKPT_BLOCK)) {}
+};
 
 unsigned grid_for(wn_context* ctx, int B) { return (unsigned)std::min<long long>(B, (long long)ctx->numCU * 32); }
 
@@ -201,8 +204,10 @@ int wn_forward_routed(wn_context* ctx, const double* X_dev, int B, int R, int C,
         if (!X_dev || !Y_dev) return fail(ctx, WN_ERR_ARG, "null pointer");
         if (!q_dev != !scale_dev) return fail(ctx, WN_ERR_ARG, "a checkpoint is values and scales");
         if (!wn::aligned_to(X_dev, 8) || !wn::aligned_to(Y_dev, 8) || !wn::aligned_to(scale_dev, 4)) return fail(ctx, WN_ERR_ARG, "misaligned pointer");
-        const size_t bytes = ((size_t)B << (A.lgR + A.lgC)) * sizeof(double);
-        if (overlap(Y_dev, bytes, X_dev, bytes)) return fail(ctx, WN_ERR_ARG, "the coefficients overlap the examples");
+        const BankMemory M(A);
+        rc = wn::refuse_overlaps(ctx, {{"Y", Y_dev, M.values * 8}, {"q", q_dev, M.values}, {"scale", scale_dev, M.blocks * 4}},
+                                 {{"X", X_dev, M.values * 8}, {"filters", filters_dev, M.bank * 8}, {"idx", idx_dev, M.entries * 4}, {"w", w_dev, M.entries * 8}});
+        if (rc) return rc;
         A.X = X_dev; A.Y = Y_dev; A.q_out = q_dev; A.qs_out = scale_dev;
         return launch_bank(ctx, NP, sc, 0, A);
     });
@@ -224,9 +229,14 @@ int wn_backprop_routed(wn_context* ctx, const double* Delta_dev, const double* X
             if (!wn::aligned_to(Delta_dev, 8) || !wn::aligned_to(X_dev, 8) || !wn::aligned_to(scale_dev, 4) || !wn::aligned_to(grad_dev, 8) ||
                 !wn::aligned_to(dw_dev, 8) || !wn::aligned_to(dX_dev, 8))
                 return fail(ctx, WN_ERR_ARG, "misaligned pointer");
-            const size_t bytes = ((size_t)B << (A.lgR + A.lgC)) * sizeof(double);
-            if (overlap(dX_dev, bytes, Delta_dev, bytes) || overlap(dX_dev, bytes, X_dev, bytes) || overlap(dX_dev, bytes, q_dev, bytes / 8))
-                return fail(ctx, WN_ERR_ARG, "the errors on the input overlap what they come from");
+        }
+        const BankMemory M(A);
+        rc = wn::refuse_overlaps(ctx, {{"grad", grad_dev, M.entries * N * 8}, {"dfilters", dfilters_dev, M.bank * 8}, {"dw", dw_dev, M.entries * 8},
+                                       {"dX", dX_dev, M.values * 8}},
+                                 {{"Delta", Delta_dev, M.values * 8}, {"X", X_dev, M.values * 8}, {"q", q_dev, M.values}, {"scale", scale_dev, M.blocks * 4},
+                                  {"filters", filters_dev, M.bank * 8}, {"idx", idx_dev, M.entries * 4}, {"w", w_dev, M.entries * 8}});
+        if (rc) return rc;
+        if (B > 0) {
             A.D = Delta_dev; A.X = X_dev; A.q = q_dev; A.qs = scale_dev; A.grad = grad_dev; A.dw = dw_dev; A.dX = dX_dev;
             rc = launch_bank(ctx, NP, sc, q_dev ? 2 : 1, A);
             if (rc) return rc;
