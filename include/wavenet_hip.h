@@ -287,14 +287,15 @@ typedef struct wn_routing {
  *     counts[f] (counts_dev may be NULL) = number of entries of idx that name f
  * A filter whose s or c is -inf (or whose bias is NaN) is closed to the row; where fewer than k are open the entries left
  * over have idx -1 and weight 0.  A row with a NaN or +inf among its s has no answer: idx -1 and weights NaN throughout
- * (and wn_forward_routed then makes its coefficients NaN).  Computed in 64 bits.
+ * (and wn_forward_routed then makes its coefficients NaN).  Computed in 64 bits.  No output may overlap an input or another
+ * output.
  */
 int wn_route(wn_context* ctx, const void* scores_dev, int dtype, int T, int F, long long row_stride, long long col_stride,
              const wn_routing* routing, const double* bias_dev, int* idx_dev, double* w_dev, int* counts_dev);
 /*
  * dw_dev[T][k]: gradient of the weights -> dscores_dev, the gradient of the scores, in the type and at the strides of the
- * scores (it may be the same memory).  idx_dev as wn_route left it: the choice itself has no gradient, nor has the bias.
- * Entries of idx outside 0 ... F - 1 count for nothing; a row without any gets zeros.
+ * scores (every one on its own score, or on none).  idx_dev as wn_route left it: the choice itself has no gradient, nor has
+ * the bias.  Entries of idx outside 0 ... F - 1 count for nothing; a row without any gets zeros.
  */
 int wn_route_backward(wn_context* ctx, const void* scores_dev, int dtype, int T, int F, long long row_stride, long long col_stride,
                       const wn_routing* routing, const int* idx_dev, const double* dw_dev, void* dscores_dev);
@@ -304,7 +305,8 @@ int wn_route_backward(wn_context* ctx, const void* scores_dev, int dtype, int T,
  * scale_dev[B][ceil(n / 64)] holds each block's largest magnitude / 127 rounded to float, q_dev[B][n] the whole number
  * nearest to value / scale (ties to even, within -127 ... 127).  A value reads back as q * scale, at most half a scale
  * off (more below a scale of 2^-126, where floats are coarser).  A block with a value that is not finite, or too large for
- * a float scale, reads back as NaN.  dtype and row_stride (elements between rows) describe X_dev.
+ * a float scale, reads back as NaN.  dtype and row_stride (elements between rows) describe X_dev.  Values and checkpoint may
+ * not overlap.
  */
 int wn_checkpoint_pack(wn_context* ctx, const void* X_dev, int dtype, int B, int n, long long row_stride, signed char* q_dev,
                        float* scale_dev);

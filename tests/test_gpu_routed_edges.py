@@ -221,3 +221,71 @@ def test_every_output_over_every_other_argument_is_refused(ctx, from_checkpoint)
         torch.cuda.synchronize()
         assert torch.equal(arena, before)
     assert tried >= 3 * 3 * 6 and used <= arena.numel()
+
+
+def test_router_and_checkpoint_outputs_over_inputs_are_refused(ctx):
+    import torch
+    from wavenet_amd import capi
+    rng = np.random.default_rng(3)
+    T, F_, k, gap = 4, 8, 2, 40
+    arena = dev(np.zeros(4 * T * (F_ + gap)))
+    base, row = arena.data_ptr() + 8 * T * (F_ + gap), 8 * (F_ + gap)
+    view = arena[T * (F_ + gap):2 * T * (F_ + gap)].view(T, F_ + gap)[:, :F_]
+    s = rng.standard_normal((T, F_))
+    view.copy_(dev(s))
+    idx, w, bias, counts = full((T, k), 0, torch.int32), full((T, k), 0.0, torch.float64), dev(np.zeros(F_)), full((F_,), 0, torch.int32)
+    spare = full((T, F_), 0.0, torch.float64)
+    torch.cuda.synchronize()
+
+    def refused(fn, *a, **kw):
+        before = arena.clone()
+        with pytest.raises(capi.WavenetError, match="overlap") as err:
+            fn(*a, **kw)
+        assert err.value.status == capi.WN_ERR_ARG
+        torch.cuda.synchronize()
+        assert torch.equal(arena, before)
+
+    by_rows, by_filters = dict(row_stride=F_ + gap, col_stride=1), dict(row_stride=1, col_stride=F_ + gap)
+    for strides, T_, n in ((by_rows, T, F_), (by_filters, F_, T)):
+        for at in (base, base + row + 8 * (F_ - 1), base + 3 * row, base - 8 * T_ * k + 8, base + row - 8):
+            refused(ctx.route, base, T_, n, idx.data_ptr() if T_ == T else spare.data_ptr(), at, k=k, **strides)
+        refused(ctx.route, base, T_, n, base + 2 * row + 8, w.data_ptr() if T_ == T else spare.data_ptr(), k=k, **strides)
+        refused(ctx.route, base, T_, n, spare.data_ptr(), spare.data_ptr() + 128, k=k, counts=base, **strides)
+    refused(ctx.route, base, T, F_, idx, bias.data_ptr() - 8, k=k, bias=bias, **by_rows)
+    refused(ctx.route, base, T, F_, w.data_ptr(), w.data_ptr() + 8, k=k, **by_rows)
+    refused(ctx.route, base, T, F_, idx, w, k=k, counts=idx.data_ptr() + 4 * T * k - 4, **by_rows)
+    # between the rows of the scores there is room
+    between = base + row + 8 * F_
+    ctx.route(base, T, F_, idx, between, k=k, counts=counts, **by_rows)
+    torch.cuda.synchronize()
+    ri, rw, rc = ref.route(s, k)
+    got = arena[T * (F_ + gap) + F_ + gap + F_:][:T * k].cpu().numpy().reshape(T, k)
+    assert np.array_equal(idx.cpu().numpy(), ri) and np.allclose(got, rw, rtol=2000 * 2.0 ** -53, atol=0) and np.array_equal(counts.cpu().numpy(), rc)
+
+    # gradients: on their own scores, beside them, or between the rows; not on other scores, indices or weights
+    dw = dev(rng.standard_normal((T, k)))
+    want = ref.route_backward(s, ri, dw.cpu().numpy())
+    for at in (8, -8, row, -row, 3 * row, row + 16, 8 * (F_ - 1), -2 * row + 8 * (F_ - 1)):
+        refused(ctx.route_backward, base, T, F_, idx, dw, base + at, k=k, **by_rows)
+    refused(ctx.route_backward, base, T, F_, idx, base + row + 8 * (F_ + 2), base + 16, k=k, **by_rows)
+    refused(ctx.route_backward, base, T, F_, idx, base + row + 8 * (F_ + 2), base + 8 * (F_ + 2), k=k, **by_rows)
+    refused(ctx.route_backward, base, T, F_, base + 3 * row + 8 * (F_ + 1), dw, base + 8 * F_, k=k, **by_rows)
+    for at in (8 * F_, -8 * F_, 4 * row, -4 * row):
+        out = base + at
+        ctx.route_backward(base, T, F_, idx, dw, out, k=k, **by_rows)
+        torch.cuda.synchronize()
+        first = (out - arena.data_ptr()) // 8
+        got = arena.as_strided((T, F_), (F_ + gap, 1), first).cpu().numpy()
+        assert (np.abs(got - want) <= 1e-11 * max(1.0, np.abs(want).max())).all() and np.array_equal(view.cpu().numpy(), s)
+
+    # checkpoints
+    q, sc = full((T, F_), 0, torch.int8), full((T,), 0.0, torch.float32)
+    for a in ((base, sc.data_ptr()), (base + 2 * row + 8 * F_ - 1, sc.data_ptr()), (q.data_ptr(), base + row), (q.data_ptr(), base - 12),
+              (q.data_ptr(), q.data_ptr() + T * F_ - 4)):
+        refused(ctx.checkpoint_pack, base, T, F_, *a, row_stride=F_ + gap)
+    for a in ((base, sc.data_ptr()), (q.data_ptr(), base + row)):
+        refused(ctx.checkpoint_unpack, *a, T, F_, base, row_stride=F_ + gap)
+    ctx.checkpoint_pack(base, T, F_, base + 8 * F_, base + 8 * F_ + T * F_, row_stride=F_ + gap)      # between two rows
+    ctx.checkpoint_unpack(base + 8 * F_, base + 8 * F_ + T * F_, T, F_, spare)
+    torch.cuda.synchronize()
+    assert np.array_equal(spare.cpu().numpy(), ref.unpack(*ref.pack(s))) and np.array_equal(view.cpu().numpy(), s)

@@ -117,6 +117,10 @@ int run(wn_context* ctx, bool pack, const void* wide, int dtype, int B, int n, l
     if (ld > (1LL << 40)) return wn::fail(ctx, WN_ERR_UNSUPPORTED, "rows too far apart");
     A.n = n;
     A.nb = ((unsigned)n + wn::CKPT_BLOCK - 1) / wn::CKPT_BLOCK;
+    const wn::Memory values = {"X", wide, n * es, (unsigned long long)B, ld * es}, whole = {"q", q, (unsigned long long)B * n},
+                     parts = {"scale", scales, (unsigned long long)B * A.nb * 4};
+    const int rc = pack ? wn::refuse_overlaps(ctx, {whole, parts}, {values}) : wn::refuse_overlaps(ctx, {values}, {whole, parts});
+    if (rc) return rc;
     A.ld = ld;
     const int rows = (int)std::min<long long>(B, (1LL << 31) / A.nb - 1);   // of a launch; a row has at most 2^25 blocks
     for (int first = 0; first < B; first += rows) {

@@ -9,6 +9,7 @@
 // k = 8: about 300 of these instructions; k rounds of a largest value with its number took some 1400.)  Where the bits
 // given up could have mattered, which is checked on the result, the row is chosen again by rounds on the full values.
 #include <algorithm>
+#include <cstdlib>
 
 #include "wn_bank.h"
 
@@ -1049,6 +1050,27 @@ int check_routing(wn_context* ctx, const void* scores, int dtype, int T, int F, 
     return WN_OK;
 }
 
+// The memory of scores, or of their gradients, as pieces of the direction whose elements lie closer together.
+wn::Memory score_memory(const char* name, const void* at, const wn::RouteArgs& A) {
+    const unsigned long long es = wn::element_bytes(A.dtype);
+    const bool rows_outside = A.T == 1 || (A.F > 1 ? A.rs > A.cs : true);
+    const unsigned long long inner = rows_outside ? (A.F - 1) * A.cs + 1 : (A.T - 1) * A.rs + 1;
+    return {name, at, inner * es, (unsigned long long)(rows_outside ? A.T : A.F), (unsigned long long)(rows_outside ? A.rs : A.cs) * es};
+}
+// Whether gradients `by` elements behind the scores, at the same strides, lie on scores other than their own.
+bool on_other_scores(long long by, const wn::RouteArgs& A) {
+    if (by < 0) by = -by;
+    const bool rows_outside = A.T == 1 || (A.F > 1 ? A.rs > A.cs : true);
+    // outer and inner stride and counts: (T or F) pieces of (F or T) elements
+    const long long so = rows_outside ? A.rs : A.cs, no = rows_outside ? A.T : A.F;
+    const long long si = rows_outside ? A.cs : A.rs, ni = rows_outside ? A.F : A.T;
+    if (by == 0) return false;
+    const auto inside = [&](long long d) { return d == 0 || (ni > 1 && d % si == 0 && std::abs(d / si) < ni); };
+    if (no == 1) return inside(by);
+    const long long i = by / so;                             // inner pieces are shorter than so: piece i or the next
+    return (i < no && inside(by - i * so)) || (i + 1 < no && inside(by - (i + 1) * so));
+}
+
 }  // namespace
 
 extern "C" {
@@ -1065,8 +1087,14 @@ int wn_route(wn_context* ctx, const void* scores_dev, int dtype, int T, int F, l
             if (!idx_dev || !w_dev) return fail(ctx, WN_ERR_ARG, "null pointer");
             if (!wn::aligned_to(bias_dev, 8) || !wn::aligned_to(idx_dev, 4) || !wn::aligned_to(w_dev, 8) || !wn::aligned_to(counts_dev, 4))
                 return fail(ctx, WN_ERR_ARG, "misaligned pointer");
+            const unsigned long long entries = (unsigned long long)T * A.k;
+            rc = wn::refuse_overlaps(ctx, {{"idx", idx_dev, entries * 4}, {"w", w_dev, entries * 8}, {"counts", counts_dev, 4ull * F}},
+                                     {score_memory("scores", scores_dev, A), {"bias", bias_dev, 8ull * F}});
+            if (rc) return rc;
         } else if (!counts_dev) {
             return WN_OK;
+        } else if (!wn::aligned_to(counts_dev, 4)) {
+            return fail(ctx, WN_ERR_ARG, "misaligned pointer");
         }
         const RouteClass K = route_class(F, routing->k, dtype, bias_dev, routing->groups_kept < routing->groups);
         const int rows = wn::ROUTE_T / K.lpr;
@@ -1094,6 +1122,11 @@ int wn_route_backward(wn_context* ctx, const void* scores_dev, int dtype, int T,
         if (!idx_dev || !dw_dev || !dscores_dev) return fail(ctx, WN_ERR_ARG, "null pointer");
         if (!wn::aligned_to(idx_dev, 4) || !wn::aligned_to(dw_dev, 8) || !wn::aligned_to(dscores_dev, wn::element_bytes(dtype)))
             return fail(ctx, WN_ERR_ARG, "misaligned pointer");
+        const unsigned long long entries = (unsigned long long)T * A.k;
+        rc = wn::refuse_overlaps(ctx, {score_memory("dscores", dscores_dev, A)}, {{"idx", idx_dev, entries * 4}, {"dw", dw_dev, entries * 8}});
+        if (rc) return rc;
+        const long long es = (long long)wn::element_bytes(dtype);
+        if (on_other_scores(((const char*)dscores_dev - (const char*)scores_dev) / es, A)) return fail(ctx, WN_ERR_ARG, "dscores overlaps scores of other places");
         A.idx_in = idx_dev; A.dw = dw_dev; A.dscores = dscores_dev;
         const RouteClass K = route_class(F, routing->k, dtype, false, false);
         const int rows = wn::ROUTE_T / K.lpr;
