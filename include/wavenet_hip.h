@@ -280,9 +280,11 @@ typedef struct wn_routing {
 /*
  * scores_dev: T rows of F scores of the given type, score (t, f) at t * row_stride + f * col_stride elements; no two in
  * one place.  wn_sparse_cost_grid's S_dev (filter by filter) is row_stride 1, col_stride B.
- *     s = score_scale * score;   p = softmax of the row or sigmoid(s);   c = p + bias[f] (bias_dev may be NULL)
- *     a group's score is the sum of its two largest c (the largest if there is one); the groups_kept best are kept
- *     idx[t][0 .. k): the filters of the k largest c left, largest first; equal values in order of the filter
+ *     s = score_scale * score;   p = softmax of the row or sigmoid(s);   c = p + bias[f], without bias_dev p
+ *     a group's score is the sum of its two largest c (the largest if there is one); the groups_kept best are kept, equal
+ *     ones in order of the group
+ *     idx[t][0 .. k): the filters of the k largest c left, largest first; equal values in order of the filter.  Without
+ *     bias_dev the k largest s: the same order, but shares that round to one number are told apart by their scores
  *     w[t][j] = scale * p(idx[t][j]), or with renormalise scale * p(idx[t][j]) / sum_j p(idx[t][j])
  *     counts[f] (counts_dev may be NULL) = number of entries of idx that name f
  * A filter whose s or c is -inf (or whose bias is NaN) is closed to the row; where fewer than k are open the entries left

@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 import routed_ref as ref
-from test_gpu_routed import bank_of, dev, full, host, run_backward, run_forward, run_route
+from test_gpu_routed import bank_of, dev, full, host, run_backward, run_forward, run_route, torch_type
 
 pytestmark = pytest.mark.gpu
 
@@ -69,6 +69,19 @@ def test_route_orders_the_smallest_scores(ctx, F_, k, score_scale):
         ri, rw, rc = ref.route(s, k, score_scale=score_scale, **kw)
         assert np.array_equal(idx, ri) and np.array_equal(counts, rc)
         assert np.allclose(w, rw, rtol=2000 * 2.0 ** -53, atol=0)
+
+
+@pytest.mark.parametrize("dtype", ["f64", "f32", "f16", "bf16"])
+def test_route_tells_equal_shares_apart_by_their_scores(ctx, dtype):
+    """Without a bias: sigmoids that are 1 and shares of a softmax that are 0 in 64 bits.  With one the shares are what counts."""
+    s = np.array([[40.0, 50.0, 44.0, 60.0, 48.0, 39.0, -1.0, 56.0], [-900.0, -800.0, 0.0, -850.0, -1000.0, -810.0, -950.0, -1100.0]])
+    v = dev(s, torch_type(dtype))
+    for score in ("sigmoid", "softmax"):
+        idx, _, _ = run_route(ctx, v, 4, score=score)
+        assert np.array_equal(idx, [[3, 7, 1, 4], [2, 1, 5, 3]])
+    ones = dev(np.ones(8))
+    assert np.array_equal(run_route(ctx, v, 4, score="sigmoid", bias=ones)[0][0], [0, 1, 2, 3])
+    assert np.array_equal(run_route(ctx, v, 4, bias=ones)[0][1], [2, 0, 1, 3])
 
 
 def test_route_chosen_again_in_groups_and_counted(ctx):
