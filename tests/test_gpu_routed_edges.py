@@ -84,6 +84,20 @@ def test_route_tells_equal_shares_apart_by_their_scores(ctx, dtype):
     assert np.array_equal(run_route(ctx, v, 4, bias=ones)[0][1], [2, 0, 1, 3])
 
 
+@pytest.mark.parametrize("F_,groups,kept,k", [(129, 43, 5, 9), (65, 65 // 5, 4, 6), (513, 57, 3, 16), (576, 64, 9, 16), (1000, 50, 7, 16), (33, 33, 8, 5)])
+def test_route_groups_that_end_inside_a_lane(ctx, F_, groups, kept, k):
+    """Lanes past the last filter, whose numbers would make groups past the last."""
+    rng = np.random.default_rng(F_)
+    s = rng.standard_normal((50, F_))
+    bias = rng.standard_normal(F_) * 0.05
+    for b in (None, bias):
+        for kw in (dict(score="sigmoid"), dict(renormalise=False)):
+            got = run_route(ctx, dev(s), k, groups=groups, groups_kept=kept, bias=None if b is None else dev(b), **kw)
+            want = ref.route(s, k, groups=groups, groups_kept=kept, bias=b, **kw)
+            assert np.array_equal(got[0], want[0]) and np.array_equal(got[2], want[2])
+            assert np.allclose(got[1], want[1], rtol=2000 * 2.0 ** -53, atol=0)
+
+
 def test_route_chosen_again_in_groups_and_counted(ctx):
     """Rows that the 32-bit values leave in doubt, most of a batch: the counts are those of the indices that left, and a row that
     differs from the reference holds values that 64 bits do not tell apart.  p is within 2000 * 2^-53 of itself (as the weights

@@ -392,7 +392,9 @@ __device__ __forceinline__ unsigned choose_groups(const T (&c)[VPL], T slack, co
     const unsigned long long keep = kept_groups<LPR, T>(slack, A, crow, l, doubt);
     unsigned own = 0;
 #pragma unroll
-    for (int i = 0; i < VPL; i++) own |= ((unsigned)(keep >> (((unsigned)(f0 + i) * A.per_magic) >> 20)) & 1u) << i;
+    for (int i = 0; i < VPL; i++) {                          // (lanes past the last filter may name a group past the last: closed either way)
+        own |= ((unsigned)(keep >> ((((unsigned)(f0 + i) * A.per_magic) >> 20) & 63u)) & 1u) << i;
+    }
     return own;
 }
 
