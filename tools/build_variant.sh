@@ -7,7 +7,7 @@ KIND=${KIND:-wave64}
 NPS=${NPS:-"4 8"}
 cd "$(dirname "$0")/../wavenet_amd/csrc"
 mkdir -p ../lib/exp build/exp
-FLAGS="-O3 -std=c++17 -fPIC -ffp-contract=off --offload-arch=gfx950 -I../../include -Wall -Wno-unused-result"
+FLAGS="-O3 -std=c++17 -fPIC -ffp-contract=off --offload-arch=gfx950 -I../../include -Wall -Wno-unused-result -Xclang -target-feature -Xclang -packed-fp32-ops"
 SKIP=""
 NEW=""
 if [ "$KIND" = large ]; then
