@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 import routed_ref as ref
-from test_gpu_routed import bank_of, dev, full, host, run_backward, run_forward, run_route, torch_type
+from test_gpu_routed import bank_of, dev, flat, full, host, near, run_backward, run_forward, run_route, torch_type, unflat
 
 pytestmark = pytest.mark.gpu
 
@@ -316,3 +316,43 @@ def test_router_and_checkpoint_outputs_over_inputs_are_refused(ctx):
     ctx.checkpoint_unpack(base + 8 * F_, base + 8 * F_ + T * F_, T, F_, spare)
     torch.cuda.synchronize()
     assert np.array_equal(spare.cpu().numpy(), ref.unpack(*ref.pack(s))) and np.array_equal(view.cpu().numpy(), s)
+
+
+# ---- together -------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("R,C,N,k", [(64, 64, 4, 2), (16, 32, 6, 3), (512, 1, 8, 2)])
+def test_examples_routed_by_their_costs_under_a_grid_of_filters(ctx, oracle, R, C, N, k):
+    """From wn_sparse_cost_grid's costs, filter by filter, to the gradients of the filters that suit an example best."""
+    import torch
+    rng = np.random.default_rng(R + k)
+    B, F_, n, cold = 21, 9, R * C, 0.05
+    X = rng.random((B, R, C)) ** 4
+    bank = bank_of(F_, N, 60)
+    S = full((F_, B), -1.0, torch.float64)
+    ctx.sparse_cost_grid(flat(X), B, R, C, bank, S)
+    idx, w, counts = full((B, k), -7, torch.int32), full((B, k), 7.0, torch.float64), full((F_,), -7, torch.int32)
+    how = dict(k=k, score_scale=-1.0 / cold)
+    ctx.route(S, B, F_, idx, w, row_stride=1, col_stride=B, counts=counts, **how)
+    torch.cuda.synchronize()
+    costs = S.cpu().numpy().T
+    want = np.array([[oracle.sparse_term(np.ascontiguousarray(oracle.band_forward_2d(a, x)[3].T).reshape(-1)) for a in bank] for x in X])
+    assert np.allclose(costs, want, rtol=1e-10)
+    ri, rw, rc = ref.route(costs, k, score_scale=-1.0 / cold)
+    assert np.array_equal(idx.cpu().numpy(), ri) and np.array_equal(counts.cpu().numpy(), rc)
+    assert np.allclose(w.cpu().numpy(), rw, rtol=2000 * 2.0 ** -53, atol=0)
+    assert np.array_equal(ri[:, 0], costs.argmin(axis=1))               # the sparsest comes first
+    Y, q, sc = run_forward(ctx, X, bank, ri, rw, keep=True)
+    assert near(Y, ref.forward(oracle, X, bank, ri, rw))
+    D, T = full((B, n), 7.0, torch.float64), full((B,), 7.0, torch.float64)
+    ctx.sparse_term_deriv(flat(Y), B, n, D, T)
+    torch.cuda.synchronize()
+    got = run_backward(ctx, unflat(D, R, C), bank, ri, rw, F_, N, q=q, sc=sc)
+    Xq = np.transpose(ref.unpack(*ref.pack(np.transpose(X, (0, 2, 1)).reshape(B, n))).reshape(B, C, R), (0, 2, 1))
+    for g, r in zip(got, ref.backward(oracle, unflat(D, R, C), Xq, bank, ri, rw)):
+        assert near(g, r, 1e-10)
+    assert not got[1][rc == 0].any()
+    ds = full((F_, B), 7.0, torch.float64)
+    ctx.route_backward(S, B, F_, dev(ri), dev(got[2]), ds, row_stride=1, col_stride=B, **how)
+    torch.cuda.synchronize()
+    want = ref.route_backward(costs, ri, got[2], score_scale=-1.0 / cold)
+    assert (np.abs(ds.cpu().numpy().T - want) <= 1e-10 * max(1.0, np.abs(got[2]).max()) / cold).all()
