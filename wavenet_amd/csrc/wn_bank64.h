@@ -177,7 +177,8 @@ __device__ __forceinline__ void bank_pin(double (&gL)[NP], double (&gH)[NP]) {
 // ---- kernels ----------------------------------------------------------------------------------------------
 // (An example is 32 KiB: e + gridDim.x stays far below 2^31.)
 
-// The next example's rows are on their way while this one is worked on (the registers are there, at one wave per SIMD).
+// The next example's rows are on their way while this one's columns are transformed (the registers are there, at one wave per
+// SIMD); the store of the weight and the join wait for them.
 template <int NP>
 __global__ __launch_bounds__(256, 1) void k_bank_forward64(BankArgs A) {
     extern __shared__ __attribute__((aligned(16))) double smem[];
@@ -294,7 +295,8 @@ __global__ __launch_bounds__(256, 1) void k_bank_backward64(BankArgs A) {
                 for (int i = 0; i < 64; i++) trow[i] = 0.0;
             }
             if (lane == 0) smem[waves * W64_TILE + wave] = wgt;
-            {   // the errors that come next are on their way while the results are put together
+            {   // The errors that come next are asked for before the results are put together, which waits for them (forward and
+                // backward pass of 4096 examples from the checkpoint all the same 315 -> 305 us).
                 const int next = j0 + waves < A.k ? e : e + (int)gridDim.x;
                 if (next < A.B) fetch(next);
             }

@@ -605,8 +605,8 @@ __device__ __forceinline__ unsigned bits16(bf16_bits v) { return v.v; }
 __device__ __forceinline__ unsigned bits16(float) { return 0; }
 __device__ __forceinline__ unsigned bits16(double) { return 0; }
 
-// Three waves per SIMD and as many workgroups as that makes: 65536 x 256 bf16 scores with bias and groups 52 us; two waves 55,
-// one 74, four (with spills) 93.
+// Three waves per SIMD and as many workgroups as that makes: 65536 x 256 bf16 scores with bias and groups 52 us (at 16 scores a
+// lane with 68 bytes of scratch memory per lane, 64-bit scores 120 ... 132); two waves 55, one 74, four (with more of it) 93.
 template <class S, int LPR, int VPL, int K>
 __global__ __launch_bounds__(ROUTE_T, 3) void k_route32(RouteArgs A) {
     extern __shared__ __attribute__((aligned(16))) double route_lds[];
@@ -885,7 +885,8 @@ __device__ __forceinline__ void store_chunk(const double (&ds)[VPL], const Route
 }
 
 // What the chosen filters get on their own reaches the lanes that hold them through a row of LDS that is zero otherwise.
-// Three waves per SIMD: 65536 x 256 bf16, full softmax, 45 us; two 56, four (with spills) 51.
+// Three waves per SIMD: 65536 x 256 bf16, full softmax, 43 us (at 16 scores a lane with 28 bytes of scratch memory per lane);
+// two 56, four (with more of it) 51.
 template <int LPR, int VPL>
 __global__ __launch_bounds__(ROUTE_T, 3) void k_route_backward(RouteArgs A) {
     constexpr int ROWS = ROUTE_T / LPR;
